@@ -485,6 +485,133 @@ typedef struct vxk_qweight vxk_qweight;
 VXK_API vxk_status vxk_head_logits_argmax_q(vxk_head * head, vxk_qweight * w, const float * x, int32_t rows,
                                             int32_t * argmax, float * logits, void * cuda_stream);
 
+/**
+ * Scores a batch of rows of logits: the log probability of each row's given
+ * token, the entropy of its distribution and its most likely tokens (the
+ * confidences of a transcript; the reference keeps only the argmax,
+ * src/voxtral.cpp:2966-2972).  With m = max_v l_v and s = sum_v exp(l_v - m):
+ *   logprob  = l_token - m - log s
+ *   entropy  = log s - sum_v exp(l_v - m) (l_v - m) / s          (nats)
+ *   top      = the n_top largest logits, largest first, the lowest index
+ *              first among equal ones, with their log probabilities
+ * One pass over the logits, sums in fp32.  A logit of -inf has probability 0
+ * and adds nothing to the entropy; a row with a NaN or +inf logit, or with
+ * none but -inf, has NaN outputs (its ids are then valid but mean nothing).
+ *   logits  [rows][ld] of dtype F32, F16 or BF16, device, aligned to its
+ *           element; each row's first `vocab` (the head's) elements count
+ *   tokens  [rows] int32, device: a negative one gives logprob 0 (a row that
+ *           is not scored), one >= vocab NaN and a device error at the next
+ *           vxk_head_sync
+ *   n_top   0 .. 16, at most vocab
+ *   logprob, entropy [rows] fp32, top_ids [rows][n_top] int32, top_logprobs
+ *           [rows][n_top] fp32, device; each may be NULL (tokens may be NULL
+ *           when logprob is)
+ * Asynchronous on cuda_stream.  The first scoring call of a head allocates
+ * its scratch, so make it outside a stream capture (it returns
+ * VXK_STATUS_INVALID_STATE inside one); calls of one head that overlap on the
+ * GPU race on that scratch.
+ */
+VXK_API vxk_status vxk_head_score_logits(vxk_head * head, const void * logits, vxk_dtype dtype, int64_t ld,
+                                         int32_t rows, const int32_t * tokens, int32_t n_top, float * logprob,
+                                         float * entropy, int32_t * top_ids, float * top_logprobs,
+                                         void * cuda_stream);
+
+/**
+ * vxk_head_score_logits of the logits W x[r], which are not written: the
+ * products, the softmax statistics and the top lists are one kernel, and W is
+ * read once per 2048 rows.  x is rounded to W's type as in
+ * vxk_head_logits_argmax; the tensor cores' sums are moved to fp32 registers
+ * every 512 columns.
+ *   w  [vocab][dim] f16 or bf16, device, 16-byte aligned;  x [rows][dim] fp32
+ * Everything else as in vxk_head_score_logits.
+ */
+VXK_API vxk_status vxk_head_score(vxk_head * head, const void * w, const float * x, int32_t rows,
+                                  const int32_t * tokens, int32_t n_top, float * logprob, float * entropy,
+                                  int32_t * top_ids, float * top_logprobs, void * cuda_stream);
+
+/* ======================================================================== */
+/* Packed prompts                                                           */
+/* ======================================================================== */
+
+/**
+ * Whole prompts packed behind one another, attended without a cache: the
+ * prefill graph's attention (build_decoder_prefill_graph,
+ * src/voxtral.cpp:2891-2965, with the mask of 3316-3323) for any number of
+ * sequences at once on the tensor cores, where vxk_attend_layer walks the cache
+ * once per row.  A plan names the sequences' lengths; vxk_prompt_rope turns
+ * the projections' fp32 rows into rotated 16-bit rows and
+ * vxk_prompt_attention attends within each sequence.
+ */
+typedef struct vxk_prompt vxk_prompt;
+
+typedef struct vxk_prompt_config {
+    uint32_t struct_size;
+    uint32_t api_version;
+    int32_t device;
+    int32_t n_q_heads;     /* 32; a multiple of n_kv_heads */
+    int32_t n_kv_heads;    /* 8 */
+    int32_t head_dim;      /* 64 or 128 */
+    int32_t max_seqs;      /* sequences of one plan */
+    int32_t max_rows;      /* rows of one plan, all sequences together */
+    int32_t max_position;  /* RoPE table rows: every position must be below; 0: vxk_prompt_rope is not used */
+    vxk_dtype dtype;       /* F16 or BF16: the 16-bit rows */
+    float rope_theta;      /* 1e6 */
+    float scale;           /* softmax scale; 0: 1/sqrt(head_dim) */
+    int32_t causal;        /* 1: row i attends rows <= i of its sequence; 0: every row of it */
+    int32_t window;        /* 0: none; n > 0 (causal only): row i attends rows > i - n */
+} vxk_prompt_config;
+
+/** Defaults: the decoder's heads (32/8 x 128), f16, causal, one sequence of 512 rows, positions below 8192. */
+VXK_API vxk_prompt_config vxk_prompt_default_config(void);
+VXK_API vxk_status vxk_prompt_create(const vxk_prompt_config * config, vxk_prompt ** out);
+/** NULL is safe.  No work may be in flight on it. */
+VXK_API void vxk_prompt_destroy(vxk_prompt * prompt);
+VXK_API vxk_status vxk_prompt_last_error(const vxk_prompt * prompt, char * buf, size_t capacity);
+
+/**
+ * Plans n_seqs sequences (host arrays): sequence i has n_rows[i] >= 0 rows,
+ * which follow those of sequence i - 1, at positions first_position[i] ..
+ * (NULL: from 0; they matter to vxk_prompt_rope alone).  The plan is copied to
+ * the device on cuda_stream and serves any number of calls below; a call on
+ * another stream has to be ordered behind it by the caller, as has a new plan
+ * behind the calls still using the old one.  Refused inside a stream capture.
+ * Calls captured into a graph use, at each replay, the plan of that time; a
+ * plan with more rows than the one they were captured under makes them write
+ * nothing and report a device error.
+ */
+VXK_API vxk_status vxk_prompt_plan(vxk_prompt * prompt, const int32_t * n_rows, const int32_t * first_position,
+                                   int32_t n_seqs, void * cuda_stream);
+/** Rows of the current plan. */
+VXK_API vxk_status vxk_prompt_rows(const vxk_prompt * prompt, int32_t * out_rows);
+
+/**
+ * Rotary positions and rounding of the plan's rows (RoPE mode 0: pairs
+ * (2i, 2i + 1) turned by position * theta^(-2i / head_dim), the angles in
+ * 64 bits): q, k rotated and v as it is, rounded to the prompt's type.
+ *   q [rows][n_q_heads][head_dim], k, v [rows][n_kv_heads][head_dim] fp32
+ *   q16, k16, v16 the same shapes in 16 bits
+ * Device memory, 16-byte aligned; inputs and outputs must not overlap.
+ */
+VXK_API vxk_status vxk_prompt_rope(vxk_prompt * prompt, const float * q, const float * k, const float * v, void * q16,
+                                   void * k16, void * v16, void * cuda_stream);
+
+/**
+ * Attention of every planned row within its sequence: out[i][h] =
+ * sum_j softmax_j(scale q[i][h] . k[j][h']) v[j][h'] over the rows j that row i
+ * attends (vxk_prompt_config), h' = h / (n_q_heads / n_kv_heads).  Scores,
+ * softmax and sums are fp32; the probabilities are rounded to the prompt's type
+ * for their product with v, and out is rounded once.
+ *   q, out [rows][n_q_heads][head_dim], k, v [rows][n_kv_heads][head_dim],
+ *   16-bit, device, 16-byte aligned; out overlaps no input
+ * Rows behind the plan's last are neither read for a result nor written.  No
+ * scratch: calls of one prompt may overlap.
+ */
+VXK_API vxk_status vxk_prompt_attention(vxk_prompt * prompt, const void * q, const void * k, const void * v,
+                                        void * out, void * cuda_stream);
+
+/** Bounded wait for cuda_stream, then the prompt's device error word. */
+VXK_API vxk_status vxk_prompt_sync(vxk_prompt * prompt, void * cuda_stream, int32_t timeout_ms);
+
 /* ======================================================================== */
 /* Quantized-weight matrix product (GGUF Q8_0 / Q4_K / Q6_K weights)        */
 /* ======================================================================== */

@@ -88,6 +88,12 @@ struct vxk_head {
     float * qlogits = nullptr;  // logits of the quantized path when the caller passes none
     int32_t * d_error = nullptr;
     cudaEvent_t ev_sync = nullptr;
+    // scoring scratch, allocated by the first scoring call and never moved
+    uint8_t * score = nullptr;
+    vxk::ScorePart * score_parts = nullptr;
+    int32_t * score_counters = nullptr;
+    float * score_logits = nullptr;
+    int sm_count = 0;
     CUtensorMap map_x{};
     int32_t tile_rows = 0;
     int32_t n_tiles = 0;
@@ -120,9 +126,51 @@ void free_head(vxk_head * h) {
     if (h->xh) cudaFree(h->xh);
     if (h->best) cudaFree(h->best);
     if (h->qlogits) cudaFree(h->qlogits);
+    if (h->score) cudaFree(h->score);
+    if (h->score_logits) cudaFree(h->score_logits);
     if (h->d_error) cudaFree(h->d_error);
     if (h->ev_sync) cudaEventDestroy(h->ev_sync);
     delete h;
+}
+
+// The scoring scratch of a head.  It is allocated once, at its final size, so
+// that graphs which captured scoring calls keep pointing at it.
+void need_score_scratch(vxk_head * h, cudaStream_t cs) {
+    if (h->score) return;
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    VXK_HCUDA(cudaStreamIsCapturing(cs, &st));
+    if (st != cudaStreamCaptureStatusNone)
+        hfail(VXK_STATUS_INVALID_STATE, "the first scoring call of a head allocates: make it outside a stream capture");
+    const size_t ctas = (size_t) h->sm_count * vxk::kScoreCtasPerSm;
+    const size_t parts = 2 * ctas * sizeof(vxk::ScorePart), counters = ctas * sizeof(int32_t);
+    uint8_t * base = nullptr;
+    VXK_HCUDA(cudaMalloc(&base, parts + counters));
+    if (cudaMemset(base, 0, parts + counters) != cudaSuccess) {
+        cudaFree(base);
+        hfail(VXK_STATUS_BACKEND_ERROR, "clearing the scoring scratch failed");
+    }
+    h->score_parts = reinterpret_cast<vxk::ScorePart *>(base);
+    h->score_counters = reinterpret_cast<int32_t *>(base + parts);
+    h->score = base;
+}
+
+// The outputs and checks that both scoring calls share.
+vxk::ScoreOut score_out(const vxk_head * h, int32_t rows, const int32_t * tokens, int32_t n_top, float * logprob,
+                        float * entropy, int32_t * top_ids, float * top_logprobs) {
+    if (rows < 1) hfail(VXK_STATUS_INVALID_ARGUMENT, "rows must be positive");
+    if (n_top < 0 || n_top > vxk::kMaxTop || n_top > h->cfg.vocab)
+        hfail(VXK_STATUS_INVALID_ARGUMENT, "n_top must be in [0, min(16, vocab)]");
+    if (logprob && !tokens) hfail(VXK_STATUS_INVALID_ARGUMENT, "logprob needs tokens");
+    vxk::ScoreOut o{};
+    o.tokens = logprob ? tokens : nullptr;
+    o.logprob = logprob;
+    o.entropy = entropy;
+    o.top_ids = top_ids;
+    o.top_logprobs = top_logprobs;
+    o.error = h->d_error;
+    o.n_top = top_ids || top_logprobs ? n_top : 0;
+    o.vocab = h->cfg.vocab;
+    return o;
 }
 
 }  // namespace
@@ -163,6 +211,7 @@ vxk_status vxk_head_create(const vxk_head_config * config, vxk_head ** out) {
         int sms = 0;
         VXK_HCUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device));
         if (sms < 1) hfail(VXK_STATUS_BACKEND_ERROR, "no multiprocessors");
+        h->sm_count = sms;
         const int64_t waves = std::max<int64_t>(1, ((int64_t) c.vocab + (int64_t) sms * vxk::kHeadMaxTileRows - 1) /
                                                        ((int64_t) sms * vxk::kHeadMaxTileRows));
         int64_t rows = ((int64_t) c.vocab + sms * waves - 1) / (sms * waves);
@@ -253,6 +302,82 @@ vxk_status vxk_head_logits_argmax_q(vxk_head * head, vxk_qweight * w, const floa
     });
 }
 
+vxk_status vxk_head_score_logits(vxk_head * head, const void * logits, vxk_dtype dtype, int64_t ld, int32_t rows,
+                                 const int32_t * tokens, int32_t n_top, float * logprob, float * entropy,
+                                 int32_t * top_ids, float * top_logprobs, void * cuda_stream) {
+    if (!head) return VXK_STATUS_INVALID_ARGUMENT;
+    return hguarded(head, [&] {
+        const vxk_head_config & c = head->cfg;
+        if (!logits) hfail(VXK_STATUS_INVALID_ARGUMENT, "null buffer");
+        if (dtype != VXK_DTYPE_F32 && dtype != VXK_DTYPE_F16 && dtype != VXK_DTYPE_BF16)
+            hfail(VXK_STATUS_INVALID_ARGUMENT, "logits must be F32, F16 or BF16");
+        if (ld < c.vocab) hfail(VXK_STATUS_INVALID_ARGUMENT, "ld must be at least vocab");
+        if (reinterpret_cast<uintptr_t>(logits) % (dtype == VXK_DTYPE_F32 ? 4 : 2) != 0)
+            hfail(VXK_STATUS_INVALID_ARGUMENT, "logits must be aligned to their element");
+        vxk::ScoreLogitsParams p{};
+        p.out = score_out(head, rows, tokens, n_top, logprob, entropy, top_ids, top_logprobs);
+        HeadDevice scope(c.device);
+        cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
+        need_score_scratch(head, cs);
+        p.logits = logits;
+        p.ld = ld;
+        p.rows = rows;
+        p.dtype = (int32_t) dtype;
+        p.parts = head->score_parts;
+        p.counters = head->score_counters;
+        VXK_HCUDA(vxk::launch_score_logits(p, head->sm_count, cs));
+    });
+}
+
+vxk_status vxk_head_score(vxk_head * head, const void * w, const float * x, int32_t rows, const int32_t * tokens,
+                          int32_t n_top, float * logprob, float * entropy, int32_t * top_ids, float * top_logprobs,
+                          void * cuda_stream) {
+    if (!head) return VXK_STATUS_INVALID_ARGUMENT;
+    return hguarded(head, [&] {
+        const vxk_head_config & c = head->cfg;
+        if (!w || !x) hfail(VXK_STATUS_INVALID_ARGUMENT, "null buffer");
+        if (reinterpret_cast<uintptr_t>(w) % 16 != 0) hfail(VXK_STATUS_INVALID_ARGUMENT, "w must be 16-byte aligned");
+        const vxk::ScoreOut out = score_out(head, rows, tokens, n_top, logprob, entropy, top_ids, top_logprobs);
+        HeadDevice scope(c.device);
+        cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
+        need_score_scratch(head, cs);
+        if (!head->score_logits)
+            VXK_HCUDA(cudaMalloc(&head->score_logits, (size_t) vxk::kHeadRows * c.vocab * sizeof(float)));
+        CUtensorMap map_w{};
+        encode_rows_map(&map_w, w, (int32_t) c.dtype, c.dim, c.vocab, head->tile_rows);
+        for (int32_t r0 = 0; r0 < rows; r0 += vxk::kHeadRows) {
+            vxk::HeadParams p{};
+            p.x = x + (int64_t) r0 * c.dim;
+            p.xh = head->xh;
+            p.best = head->best;
+            p.argmax = reinterpret_cast<int32_t *>(head->best);
+            p.logits = head->score_logits;
+            p.error = head->d_error;
+            p.vocab = c.vocab;
+            p.dim = c.dim;
+            p.n_rows = std::min<int32_t>(vxk::kHeadRows, rows - r0);
+            p.tile_rows = head->tile_rows;
+            p.n_tiles = head->n_tiles;
+            p.dtype = (int32_t) c.dtype;
+            VXK_HCUDA(vxk::launch_head(p, map_w, head->map_x, head->grid, cs));
+            vxk::ScoreLogitsParams q{};
+            q.logits = head->score_logits;
+            q.ld = c.vocab;
+            q.rows = p.n_rows;
+            q.dtype = VXK_DTYPE_F32;
+            q.parts = head->score_parts;
+            q.counters = head->score_counters;
+            q.out = out;
+            if (q.out.tokens) q.out.tokens += r0;
+            if (q.out.logprob) q.out.logprob += r0;
+            if (q.out.entropy) q.out.entropy += r0;
+            if (q.out.top_ids) q.out.top_ids += (int64_t) r0 * out.n_top;
+            if (q.out.top_logprobs) q.out.top_logprobs += (int64_t) r0 * out.n_top;
+            VXK_HCUDA(vxk::launch_score_logits(q, head->sm_count, cs));
+        }
+    });
+}
+
 vxk_status vxk_head_sync(vxk_head * head, void * cuda_stream, int32_t timeout_ms) {
     if (!head) return VXK_STATUS_INVALID_ARGUMENT;
     return hguarded(head, [&] {
@@ -276,6 +401,7 @@ vxk_status vxk_head_sync(vxk_head * head, void * cuda_stream, int32_t timeout_ms
         VXK_HCUDA(cudaMemcpy(&err, head->d_error, sizeof(err), cudaMemcpyDeviceToHost));
         if (err != 0) {
             VXK_HCUDA(cudaMemset(head->d_error, 0, sizeof(int32_t)));
+            if (err == vxk::kErrToken) hfail(VXK_STATUS_BACKEND_ERROR, "a given token lies outside the vocabulary");
             hfail(VXK_STATUS_BACKEND_ERROR, "greedy head kernel reported a device error (bounded wait expired)");
         }
     });

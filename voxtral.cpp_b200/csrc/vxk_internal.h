@@ -10,6 +10,8 @@
 
 #include <vector>
 
+#include "vxk_score.h"
+
 struct vxk_qweight;
 struct vxk_pool;
 struct vxk_enc_pool;
@@ -263,6 +265,64 @@ int head_smem_bytes();
 // largest value per row) through the per-row keys `best`.
 cudaError_t launch_head_argmax(const float * logits, int32_t rows, int32_t vocab, unsigned long long * best,
                                int32_t * argmax, cudaStream_t stream);
+
+// ---------------------------------------------------------------------------
+// Scores of rows of logits (vxk_head_score_logits, vxk_head_score)
+// ---------------------------------------------------------------------------
+
+constexpr int kScoreCtasPerSm = 2;  // CTAs of the logits kernel per multiprocessor
+
+struct ScoreLogitsParams {
+    const void * logits;   // [rows][ld] of dtype
+    int64_t ld;
+    int64_t rows;
+    int64_t strips;        // strips of a row (set by the launch)
+    int32_t dtype;         // 0 = f32, 1 = f16, 30 = bf16
+    ScorePart * parts;     // [2 x kScoreCtasPerSm x SMs]
+    int32_t * counters;    // [kScoreCtasPerSm x SMs], zero between launches
+    ScoreOut out;
+};
+
+cudaError_t launch_score_logits(ScoreLogitsParams p, int sms, cudaStream_t stream);
+
+// ---------------------------------------------------------------------------
+// Packed prompts (vxk_prompt_*)
+// ---------------------------------------------------------------------------
+
+constexpr int32_t kErrPlan = 5;  // device error word: the plan holds more rows than the call's buffers
+
+struct PromptRopeParams {
+    const uint8_t * plan;        // int4 {0, rows, sequences, 0} of the plan
+    const int32_t * positions;   // [rows]
+    const float2 * table;        // [max_position][head_dim / 2] (cos, sin)
+    int32_t rows;                // rows of the call's buffers
+    int32_t n_q, n_kv, head_dim, dtype;
+    const float * q;
+    const float * k;
+    const float * v;
+    uint16_t * q16;
+    uint16_t * k16;
+    uint16_t * v16;
+    int32_t * error;
+};
+
+struct PromptAttnParams {
+    const uint8_t * plan;
+    const int4 * row_seq;        // [rows] {first row of the row's sequence, its rows, 0, 0}
+    int32_t rows;
+    int32_t n_q, n_kv, head_dim, dtype;
+    int32_t causal, window;
+    float scale_log2;            // softmax scale * log2(e)
+    const void * q;
+    const void * k;
+    const void * v;
+    void * out;
+    int32_t * error;
+};
+
+cudaError_t launch_rope_table(float2 * table, int32_t rows, int32_t head_dim, double log_theta, cudaStream_t stream);
+cudaError_t launch_prompt_rope(const PromptRopeParams & p, cudaStream_t stream);
+cudaError_t launch_prompt_attention(const PromptAttnParams & p, cudaStream_t stream);
 
 // ---------------------------------------------------------------------------
 // Quantized-weight matrix product (vxk_qweight_*)

@@ -1,0 +1,355 @@
+// Host runtime of packed prompts (include/vxk.h, vxk_prompt_*): the plan of a
+// batch of sequences and the launches over it.
+#include "vxk.h"
+#include "vxk_internal.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <chrono>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <string>
+#include <thread>
+#include <vector>
+
+namespace {
+
+thread_local std::string g_prompt_create_error;
+
+struct PromptError {
+    vxk_status status;
+    std::string message;
+};
+
+[[noreturn]] void pfail(vxk_status s, const std::string & m) { throw PromptError{s, m}; }
+
+#define VXK_PCUDA(expr)                                                                 \
+    do {                                                                                \
+        const cudaError_t e_ = (expr);                                                  \
+        if (e_ != cudaSuccess) {                                                        \
+            pfail(e_ == cudaErrorMemoryAllocation ? VXK_STATUS_OUT_OF_MEMORY            \
+                                                  : VXK_STATUS_BACKEND_ERROR,           \
+                  std::string(#expr) + ": " + cudaGetErrorString(e_));                  \
+        }                                                                               \
+    } while (0)
+
+class PromptDevice {
+public:
+    explicit PromptDevice(int d) {
+        cudaGetDevice(&prev_);
+        dev_ = d;
+        if (prev_ != d) cudaSetDevice(d);
+    }
+    ~PromptDevice() {
+        if (prev_ != dev_) cudaSetDevice(prev_);
+    }
+
+private:
+    int prev_ = 0, dev_ = 0;
+};
+
+size_t align16(size_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+
+struct vxk_prompt {
+    vxk_prompt_config cfg{};
+    float2 * table = nullptr;
+    uint8_t * d_plan = nullptr;
+    uint8_t * h_plan[2] = {nullptr, nullptr};
+    cudaEvent_t plan_ev[2] = {nullptr, nullptr};
+    int plan_next = 0;
+    size_t plan_bytes = 0;
+    size_t off_positions = 0;   // offsets into the plan
+    size_t off_row_seq = 0;
+    int32_t * d_error = nullptr;
+    cudaEvent_t ev_sync = nullptr;
+    int sm_count = 0;
+    int32_t rows = -1;          // rows of the current plan, -1 before the first
+    std::string last_error;
+};
+
+namespace {
+
+template <typename F>
+vxk_status pguarded(vxk_prompt * p, F && body) {
+    try {
+        body();
+        return VXK_STATUS_OK;
+    } catch (const PromptError & e) {
+        if (p) p->last_error = e.message;
+        return e.status;
+    } catch (const std::bad_alloc &) {
+        if (p) p->last_error = "host out of memory";
+        return VXK_STATUS_OUT_OF_MEMORY;
+    } catch (...) {
+        if (p) p->last_error = "internal error";
+        return VXK_STATUS_INTERNAL_ERROR;
+    }
+}
+
+void free_prompt(vxk_prompt * p) {
+    if (!p) return;
+    PromptDevice scope(p->cfg.device);
+    if (p->table) cudaFree(p->table);
+    if (p->d_plan) cudaFree(p->d_plan);
+    for (int i = 0; i < 2; ++i) {
+        if (p->h_plan[i]) cudaFreeHost(p->h_plan[i]);
+        if (p->plan_ev[i]) cudaEventDestroy(p->plan_ev[i]);
+    }
+    if (p->d_error) cudaFree(p->d_error);
+    if (p->ev_sync) cudaEventDestroy(p->ev_sync);
+    delete p;
+}
+
+void check_config(const vxk_prompt_config & c) {
+    if (c.struct_size < sizeof(vxk_prompt_config)) pfail(VXK_STATUS_INVALID_ARGUMENT, "config struct_size too small");
+    if (c.head_dim != 64 && c.head_dim != 128) pfail(VXK_STATUS_INVALID_ARGUMENT, "head_dim must be 64 or 128");
+    if (c.n_kv_heads < 1 || c.n_q_heads < 1 || c.n_q_heads % c.n_kv_heads != 0 || c.n_q_heads > 1024)
+        pfail(VXK_STATUS_INVALID_ARGUMENT, "n_q_heads must be a multiple of n_kv_heads, at most 1024");
+    if (c.max_seqs < 1 || c.max_seqs > (1 << 20)) pfail(VXK_STATUS_INVALID_ARGUMENT, "max_seqs must be in [1, 2^20]");
+    if (c.max_rows < 1 || c.max_rows > (1 << 22)) pfail(VXK_STATUS_INVALID_ARGUMENT, "max_rows must be in [1, 2^22]");
+    if (c.max_position < 0) pfail(VXK_STATUS_INVALID_ARGUMENT, "max_position must not be negative");
+    if (c.dtype != VXK_DTYPE_F16 && c.dtype != VXK_DTYPE_BF16)
+        pfail(VXK_STATUS_INVALID_ARGUMENT, "the prompt's type must be F16 or BF16");
+    if (!(c.rope_theta > 0.0f) || !std::isfinite(c.rope_theta))
+        pfail(VXK_STATUS_INVALID_ARGUMENT, "rope_theta must be positive");
+    if (!(c.scale >= 0.0f) || !std::isfinite(c.scale))
+        pfail(VXK_STATUS_INVALID_ARGUMENT, "scale must be positive, or 0 for 1/sqrt(head_dim)");
+    if (c.causal != 0 && c.causal != 1) pfail(VXK_STATUS_INVALID_ARGUMENT, "causal must be 0 or 1");
+    if (c.window < 0 || (c.window > 0 && !c.causal))
+        pfail(VXK_STATUS_INVALID_ARGUMENT, "window must not be negative and needs causal");
+}
+
+void check_capture(cudaStream_t cs, const char * what) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    VXK_PCUDA(cudaStreamIsCapturing(cs, &st));
+    if (st != cudaStreamCaptureStatusNone) pfail(VXK_STATUS_INVALID_STATE, std::string(what) + " inside a stream capture");
+}
+
+void check_buffers(const vxk_prompt * p, std::initializer_list<const void *> ptrs) {
+    if (p->rows < 0) pfail(VXK_STATUS_INVALID_STATE, "no plan");
+    for (const void * a : ptrs) {
+        if (!a) pfail(VXK_STATUS_INVALID_ARGUMENT, "null buffer");
+        if (reinterpret_cast<uintptr_t>(a) % 16 != 0)
+            pfail(VXK_STATUS_INVALID_ARGUMENT, "buffers must be 16-byte aligned");
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+vxk_prompt_config vxk_prompt_default_config(void) {
+    vxk_prompt_config c{};
+    c.struct_size = sizeof(vxk_prompt_config);
+    c.api_version = VXK_API_VERSION;
+    c.n_q_heads = 32;
+    c.n_kv_heads = 8;
+    c.head_dim = 128;
+    c.max_seqs = 1;
+    c.max_rows = 512;
+    c.max_position = 8192;
+    c.dtype = VXK_DTYPE_F16;
+    c.rope_theta = 1000000.0f;
+    c.causal = 1;
+    return c;
+}
+
+vxk_status vxk_prompt_create(const vxk_prompt_config * config, vxk_prompt ** out) {
+    if (out) *out = nullptr;
+    if (!config || !out) {
+        g_prompt_create_error = "null argument";
+        return VXK_STATUS_INVALID_ARGUMENT;
+    }
+    vxk_prompt * p = new (std::nothrow) vxk_prompt();
+    if (!p) return VXK_STATUS_OUT_OF_MEMORY;
+    const vxk_status st = pguarded(p, [&] {
+        const vxk_prompt_config & c = *config;
+        check_config(c);
+        p->cfg = c;
+        int n_dev = 0;
+        VXK_PCUDA(cudaGetDeviceCount(&n_dev));
+        if (c.device < 0 || c.device >= n_dev) {
+            p->cfg.device = 0;
+            pfail(VXK_STATUS_INVALID_ARGUMENT, "no such CUDA device");
+        }
+        PromptDevice scope(c.device);
+        VXK_PCUDA(cudaDeviceGetAttribute(&p->sm_count, cudaDevAttrMultiProcessorCount, c.device));
+        p->off_positions = 16;
+        p->off_row_seq = p->off_positions + align16((size_t) c.max_rows * sizeof(int32_t));
+        p->plan_bytes = p->off_row_seq + (size_t) c.max_rows * sizeof(int4);
+        VXK_PCUDA(cudaMalloc(&p->d_plan, p->plan_bytes));
+        for (int i = 0; i < 2; ++i) {
+            VXK_PCUDA(cudaHostAlloc(reinterpret_cast<void **>(&p->h_plan[i]), p->plan_bytes, cudaHostAllocDefault));
+            VXK_PCUDA(cudaEventCreateWithFlags(&p->plan_ev[i], cudaEventDisableTiming));
+        }
+        VXK_PCUDA(cudaMalloc(&p->d_error, sizeof(int32_t)));
+        VXK_PCUDA(cudaMemset(p->d_error, 0, sizeof(int32_t)));
+        VXK_PCUDA(cudaEventCreateWithFlags(&p->ev_sync, cudaEventDisableTiming));
+        if (c.max_position > 0) {
+            VXK_PCUDA(cudaMalloc(&p->table, (size_t) c.max_position * (c.head_dim / 2) * sizeof(float2)));
+            VXK_PCUDA(vxk::launch_rope_table(p->table, c.max_position, c.head_dim, std::log((double) c.rope_theta),
+                                             nullptr));
+            VXK_PCUDA(cudaStreamSynchronize(nullptr));
+        }
+    });
+    if (st != VXK_STATUS_OK) {
+        g_prompt_create_error = p->last_error;
+        free_prompt(p);
+        return st;
+    }
+    *out = p;
+    return VXK_STATUS_OK;
+}
+
+void vxk_prompt_destroy(vxk_prompt * prompt) { free_prompt(prompt); }
+
+vxk_status vxk_prompt_last_error(const vxk_prompt * prompt, char * buf, size_t capacity) {
+    if (!buf || capacity == 0) return VXK_STATUS_INVALID_ARGUMENT;
+    const std::string & m = prompt ? prompt->last_error : g_prompt_create_error;
+    const size_t n = std::min(capacity - 1, m.size());
+    std::memcpy(buf, m.data(), n);
+    buf[n] = '\0';
+    return m.size() < capacity ? VXK_STATUS_OK : VXK_STATUS_BUFFER_TOO_SMALL;
+}
+
+vxk_status vxk_prompt_plan(vxk_prompt * prompt, const int32_t * n_rows, const int32_t * first_position,
+                           int32_t n_seqs, void * cuda_stream) {
+    if (!prompt) return VXK_STATUS_INVALID_ARGUMENT;
+    return pguarded(prompt, [&] {
+        const vxk_prompt_config & c = prompt->cfg;
+        if (!n_rows || n_seqs < 1 || n_seqs > c.max_seqs)
+            pfail(VXK_STATUS_INVALID_ARGUMENT, "n_seqs must be in [1, max_seqs]");
+        int64_t total = 0;
+        for (int32_t i = 0; i < n_seqs; ++i) {
+            const int64_t first = first_position ? first_position[i] : 0;
+            if (n_rows[i] < 0 || first < 0) pfail(VXK_STATUS_INVALID_ARGUMENT, "negative rows or position");
+            if (c.max_position > 0 && n_rows[i] > 0 && first + n_rows[i] > c.max_position)
+                pfail(VXK_STATUS_INVALID_ARGUMENT, "a position reaches max_position");
+            total += n_rows[i];
+        }
+        if (total > c.max_rows) pfail(VXK_STATUS_INVALID_ARGUMENT, "the plan has more than max_rows rows");
+        PromptDevice scope(c.device);
+        cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
+        check_capture(cs, "vxk_prompt_plan");
+        const int slot = prompt->plan_next;
+        VXK_PCUDA(cudaEventSynchronize(prompt->plan_ev[slot]));
+        uint8_t * h = prompt->h_plan[slot];
+        const int32_t head[4] = {0, (int32_t) total, n_seqs, 0};
+        std::memcpy(h, head, sizeof(head));
+        int32_t * pos = reinterpret_cast<int32_t *>(h + prompt->off_positions);
+        int4 * seq = reinterpret_cast<int4 *>(h + prompt->off_row_seq);
+        int32_t row = 0;
+        for (int32_t i = 0; i < n_seqs; ++i) {
+            const int32_t row0 = row;
+            for (int32_t j = 0; j < n_rows[i]; ++j, ++row) {
+                pos[row] = (first_position ? first_position[i] : 0) + j;
+                seq[row] = make_int4(row0, n_rows[i], 0, 0);
+            }
+        }
+        VXK_PCUDA(cudaMemcpyAsync(prompt->d_plan, h, prompt->plan_bytes, cudaMemcpyHostToDevice, cs));
+        VXK_PCUDA(cudaEventRecord(prompt->plan_ev[slot], cs));
+        prompt->plan_next ^= 1;
+        prompt->rows = (int32_t) total;
+    });
+}
+
+vxk_status vxk_prompt_rows(const vxk_prompt * prompt, int32_t * out_rows) {
+    if (!prompt || !out_rows) return VXK_STATUS_INVALID_ARGUMENT;
+    if (prompt->rows < 0) return VXK_STATUS_INVALID_STATE;
+    *out_rows = prompt->rows;
+    return VXK_STATUS_OK;
+}
+
+vxk_status vxk_prompt_rope(vxk_prompt * prompt, const float * q, const float * k, const float * v, void * q16,
+                           void * k16, void * v16, void * cuda_stream) {
+    if (!prompt) return VXK_STATUS_INVALID_ARGUMENT;
+    return pguarded(prompt, [&] {
+        const vxk_prompt_config & c = prompt->cfg;
+        if (c.max_position == 0) pfail(VXK_STATUS_INVALID_STATE, "the prompt was created without positions");
+        check_buffers(prompt, {q, k, v, q16, k16, v16});
+        if (prompt->rows == 0) return;
+        PromptDevice scope(c.device);
+        vxk::PromptRopeParams a{};
+        a.plan = prompt->d_plan;
+        a.positions = reinterpret_cast<const int32_t *>(prompt->d_plan + prompt->off_positions);
+        a.table = prompt->table;
+        a.rows = prompt->rows;
+        a.n_q = c.n_q_heads;
+        a.n_kv = c.n_kv_heads;
+        a.head_dim = c.head_dim;
+        a.dtype = (int32_t) c.dtype;
+        a.q = q;
+        a.k = k;
+        a.v = v;
+        a.q16 = static_cast<uint16_t *>(q16);
+        a.k16 = static_cast<uint16_t *>(k16);
+        a.v16 = static_cast<uint16_t *>(v16);
+        a.error = prompt->d_error;
+        VXK_PCUDA(vxk::launch_prompt_rope(a, static_cast<cudaStream_t>(cuda_stream)));
+    });
+}
+
+vxk_status vxk_prompt_attention(vxk_prompt * prompt, const void * q, const void * k, const void * v, void * out,
+                                void * cuda_stream) {
+    if (!prompt) return VXK_STATUS_INVALID_ARGUMENT;
+    return pguarded(prompt, [&] {
+        const vxk_prompt_config & c = prompt->cfg;
+        check_buffers(prompt, {q, k, v, out});
+        if (prompt->rows == 0) return;
+        PromptDevice scope(c.device);
+        vxk::PromptAttnParams a{};
+        a.plan = prompt->d_plan;
+        a.row_seq = reinterpret_cast<const int4 *>(prompt->d_plan + prompt->off_row_seq);
+        a.rows = prompt->rows;
+        a.n_q = c.n_q_heads;
+        a.n_kv = c.n_kv_heads;
+        a.head_dim = c.head_dim;
+        a.dtype = (int32_t) c.dtype;
+        a.causal = c.causal;
+        a.window = c.window;
+        const double scale = c.scale > 0.0f ? (double) c.scale : 1.0 / std::sqrt((double) c.head_dim);
+        a.scale_log2 = (float) (scale * 1.4426950408889634);
+        a.q = q;
+        a.k = k;
+        a.v = v;
+        a.out = out;
+        a.error = prompt->d_error;
+        VXK_PCUDA(vxk::launch_prompt_attention(a, static_cast<cudaStream_t>(cuda_stream)));
+    });
+}
+
+vxk_status vxk_prompt_sync(vxk_prompt * prompt, void * cuda_stream, int32_t timeout_ms) {
+    if (!prompt) return VXK_STATUS_INVALID_ARGUMENT;
+    return pguarded(prompt, [&] {
+        PromptDevice scope(prompt->cfg.device);
+        VXK_PCUDA(cudaEventRecord(prompt->ev_sync, static_cast<cudaStream_t>(cuda_stream)));
+        const auto t0 = std::chrono::steady_clock::now();
+        while (true) {
+            const cudaError_t e = cudaEventQuery(prompt->ev_sync);
+            if (e == cudaSuccess) break;
+            if (e != cudaErrorNotReady) pfail(VXK_STATUS_BACKEND_ERROR, cudaGetErrorString(e));
+            const auto ms =
+                std::chrono::duration_cast<std::chrono::milliseconds>(std::chrono::steady_clock::now() - t0).count();
+            if (ms > timeout_ms) pfail(VXK_STATUS_TIMEOUT, "stream did not drain within the timeout");
+            // poll short waits; sleep between polls after 20 ms
+            if (ms < 20)
+                std::this_thread::yield();
+            else
+                std::this_thread::sleep_for(std::chrono::microseconds(50));
+        }
+        int32_t err = 0;
+        VXK_PCUDA(cudaMemcpy(&err, prompt->d_error, sizeof(err), cudaMemcpyDeviceToHost));
+        if (err != 0) {
+            VXK_PCUDA(cudaMemset(prompt->d_error, 0, sizeof(int32_t)));
+            if (err == vxk::kErrPlan)
+                pfail(VXK_STATUS_BACKEND_ERROR, "a replayed call met a plan of more rows than it was captured under");
+            pfail(VXK_STATUS_BACKEND_ERROR, "prompt kernel reported a device error (bounded wait expired)");
+        }
+    });
+}
+
+}  // extern "C"

@@ -86,6 +86,14 @@ class HeadConfig(C.Structure):
                 ("dim", C.c_int32), ("vocab", C.c_int32), ("dtype", C.c_int32)]
 
 
+class PromptConfig(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("api_version", C.c_uint32), ("device", C.c_int32),
+                ("n_q_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("max_seqs", C.c_int32), ("max_rows", C.c_int32), ("max_position", C.c_int32),
+                ("dtype", C.c_int32), ("rope_theta", C.c_float), ("scale", C.c_float),
+                ("causal", C.c_int32), ("window", C.c_int32)]
+
+
 class QWeightConfig(C.Structure):
     _fields_ = [("struct_size", C.c_uint32), ("api_version", C.c_uint32), ("device", C.c_int32),
                 ("type", C.c_int32), ("n_rows", C.c_int32), ("n_cols", C.c_int32), ("max_batch", C.c_int32),
@@ -186,6 +194,17 @@ SIGNATURES = {
     "vxk_head_logits_argmax": (_I32, [_P, _P, _P, _I32, _P, _P, _P]),
     "vxk_head_sync": (_I32, [_P, _P, _I32]),
     "vxk_head_logits_argmax_q": (_I32, [_P, _P, _P, _I32, _P, _P, _P]),
+    "vxk_head_score_logits": (_I32, [_P, _P, _I32, _I64, _I32, _P, _I32, _P, _P, _P, _P, _P]),
+    "vxk_head_score": (_I32, [_P, _P, _P, _I32, _P, _I32, _P, _P, _P, _P, _P]),
+    "vxk_prompt_default_config": (PromptConfig, []),
+    "vxk_prompt_create": (_I32, [C.POINTER(PromptConfig), C.POINTER(C.c_void_p)]),
+    "vxk_prompt_destroy": (None, [_P]),
+    "vxk_prompt_last_error": (_I32, [_P, C.c_char_p, C.c_size_t]),
+    "vxk_prompt_plan": (_I32, [_P, _I32P, _I32P, _I32, _P]),
+    "vxk_prompt_rows": (_I32, [_P, _I32P]),
+    "vxk_prompt_rope": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P]),
+    "vxk_prompt_attention": (_I32, [_P, _P, _P, _P, _P, _P]),
+    "vxk_prompt_sync": (_I32, [_P, _P, _I32]),
     "vxk_qweight_default_config": (QWeightConfig, []),
     "vxk_qweight_packed_bytes": (_I32, [_I32, _I32, _I32, C.POINTER(C.c_size_t)]),
     "vxk_qweight_repack": (_I32, [_I32, _I32, _I32, _P, C.c_size_t, _P, C.c_size_t]),
@@ -505,8 +524,88 @@ class Head:
                                                       C.c_void_p(argmax_ptr), C.c_void_p(logits_ptr or None),
                                                       C.c_void_p(cuda_stream)))
 
+    def score(self, w_ptr, x_ptr, rows, tokens_ptr, n_top, logprob_ptr=0, entropy_ptr=0, top_ids_ptr=0,
+              top_logprobs_ptr=0, cuda_stream=0):
+        """Log probabilities of given tokens, entropies and top alternatives of W x (vxk_head_score)."""
+        st = self.lib.vxk_head_score(self.h, w_ptr, x_ptr, rows, tokens_ptr, n_top, logprob_ptr, entropy_ptr,
+                                     top_ids_ptr, top_logprobs_ptr, cuda_stream)
+        if st != OK:
+            raise VxkError(st, self.last_error())
+
+    def score_logits(self, logits_ptr, dtype, ld, rows, tokens_ptr, n_top, logprob_ptr=0, entropy_ptr=0,
+                     top_ids_ptr=0, top_logprobs_ptr=0, cuda_stream=0):
+        """The same from logits in memory, [rows][ld] of dtype (vxk_head_score_logits)."""
+        st = self.lib.vxk_head_score_logits(self.h, logits_ptr, dtype, ld, rows, tokens_ptr, n_top, logprob_ptr,
+                                            entropy_ptr, top_ids_ptr, top_logprobs_ptr, cuda_stream)
+        if st != OK:
+            raise VxkError(st, self.last_error())
+
     def sync(self, cuda_stream=0, timeout_ms=10000):
         self._check(self.lib.vxk_head_sync(self.h, C.c_void_p(cuda_stream), timeout_ms))
+
+
+class Prompt:
+    """Owns one vxk_prompt (packed prompts: rotary rows and attention within
+    each sequence, on one device)."""
+
+    def __init__(self, **cfg):
+        self.lib = load()
+        c = self.lib.vxk_prompt_default_config()
+        for k, v in cfg.items():
+            if not hasattr(c, k):
+                raise AttributeError(k)
+            setattr(c, k, v)
+        self.config = c
+        h = C.c_void_p()
+        st = self.lib.vxk_prompt_create(C.byref(c), C.byref(h))
+        if st != OK:
+            raise VxkError(st, self.last_error(None))
+        self.h = h
+
+    def last_error(self, handle="self") -> str:
+        buf = C.create_string_buffer(1024)
+        hv = self.h if handle == "self" else handle
+        self.lib.vxk_prompt_last_error(hv, buf, 1024)
+        return buf.value.decode()
+
+    def _check(self, st):
+        if st != OK:
+            raise VxkError(st, self.last_error())
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.lib.vxk_prompt_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def plan(self, n_rows, first_position=None, cuda_stream=0) -> int:
+        """Plans sequences of n_rows[i] rows from first_position[i] (0 when None); returns the rows of all."""
+        n = list(n_rows)
+        first = _i32_array(list(first_position)) if first_position is not None else None
+        if first is not None and len(first) != len(n):
+            raise VxkError(INVALID_ARGUMENT, "one first position per sequence is needed")
+        self._check(self.lib.vxk_prompt_plan(self.h, _i32_array(n), first, len(n), C.c_void_p(cuda_stream)))
+        rows = C.c_int32()
+        self._check(self.lib.vxk_prompt_rows(self.h, C.byref(rows)))
+        return rows.value
+
+    def rope(self, q_ptr, k_ptr, v_ptr, q16_ptr, k16_ptr, v16_ptr, cuda_stream=0):
+        st = self.lib.vxk_prompt_rope(self.h, q_ptr, k_ptr, v_ptr, q16_ptr, k16_ptr, v16_ptr, cuda_stream)
+        if st != OK:
+            raise VxkError(st, self.last_error())
+
+    def attention(self, q_ptr, k_ptr, v_ptr, out_ptr, cuda_stream=0):
+        st = self.lib.vxk_prompt_attention(self.h, q_ptr, k_ptr, v_ptr, out_ptr, cuda_stream)
+        if st != OK:
+            raise VxkError(st, self.last_error())
+
+    def sync(self, cuda_stream=0, timeout_ms=10000):
+        self._check(self.lib.vxk_prompt_sync(self.h, C.c_void_p(cuda_stream), timeout_ms))
 
 
 # ---- planners (host only) -------------------------------------------------
