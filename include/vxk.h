@@ -521,7 +521,7 @@ VXK_API vxk_status vxk_head_score_logits(vxk_head * head, const void * logits, v
  * products, the softmax statistics and the top lists are one kernel, and W is
  * read once per 2048 rows.  x is rounded to W's type as in
  * vxk_head_logits_argmax; the tensor cores' sums are moved to fp32 registers
- * every 512 columns.
+ * every 256 columns.
  *   w  [vocab][dim] f16 or bf16, device, 16-byte aligned;  x [rows][dim] fp32
  * Everything else as in vxk_head_score_logits.
  */

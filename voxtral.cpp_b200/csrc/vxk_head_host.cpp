@@ -92,7 +92,11 @@ struct vxk_head {
     uint8_t * score = nullptr;
     vxk::ScorePart * score_parts = nullptr;
     int32_t * score_counters = nullptr;
-    float * score_logits = nullptr;
+    uint16_t * score_xh = nullptr;
+    float4 * score_stats = nullptr;
+    unsigned long long * score_keys = nullptr;
+    float * score_tokens = nullptr;
+    uint32_t * score_low = nullptr;
     int sm_count = 0;
     CUtensorMap map_x{};
     int32_t tile_rows = 0;
@@ -127,7 +131,6 @@ void free_head(vxk_head * h) {
     if (h->best) cudaFree(h->best);
     if (h->qlogits) cudaFree(h->qlogits);
     if (h->score) cudaFree(h->score);
-    if (h->score_logits) cudaFree(h->score_logits);
     if (h->d_error) cudaFree(h->d_error);
     if (h->ev_sync) cudaEventDestroy(h->ev_sync);
     delete h;
@@ -142,15 +145,30 @@ void need_score_scratch(vxk_head * h, cudaStream_t cs) {
     if (st != cudaStreamCaptureStatusNone)
         hfail(VXK_STATUS_INVALID_STATE, "the first scoring call of a head allocates: make it outside a stream capture");
     const size_t ctas = (size_t) h->sm_count * vxk::kScoreCtasPerSm;
-    const size_t parts = 2 * ctas * sizeof(vxk::ScorePart), counters = ctas * sizeof(int32_t);
+    const size_t slots = (size_t) h->sm_count * 2 * 128;  // rows of all epilogue halves
+    size_t at = 0;
+    auto take = [&at](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const size_t counters = take(ctas * sizeof(int32_t)), parts = take(2 * ctas * sizeof(vxk::ScorePart));
+    const size_t stats = take(slots * sizeof(float4)), keys = take(slots * vxk::kMaxTop * 8);
+    const size_t tokens = take(vxk::kScoreRows * sizeof(float)), low = take(vxk::kScoreRows * sizeof(uint32_t));
+    const size_t xh = take((size_t) vxk::kScoreRows * h->cfg.dim * 2);
     uint8_t * base = nullptr;
-    VXK_HCUDA(cudaMalloc(&base, parts + counters));
-    if (cudaMemset(base, 0, parts + counters) != cudaSuccess) {
+    VXK_HCUDA(cudaMalloc(&base, at));
+    if (cudaMemset(base, 0, ctas * sizeof(int32_t)) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess) {
         cudaFree(base);
         hfail(VXK_STATUS_BACKEND_ERROR, "clearing the scoring scratch failed");
     }
-    h->score_parts = reinterpret_cast<vxk::ScorePart *>(base);
-    h->score_counters = reinterpret_cast<int32_t *>(base + parts);
+    h->score_counters = reinterpret_cast<int32_t *>(base + counters);
+    h->score_parts = reinterpret_cast<vxk::ScorePart *>(base + parts);
+    h->score_stats = reinterpret_cast<float4 *>(base + stats);
+    h->score_keys = reinterpret_cast<unsigned long long *>(base + keys);
+    h->score_tokens = reinterpret_cast<float *>(base + tokens);
+    h->score_low = reinterpret_cast<uint32_t *>(base + low);
+    h->score_xh = reinterpret_cast<uint16_t *>(base + xh);
     h->score = base;
 }
 
@@ -341,39 +359,37 @@ vxk_status vxk_head_score(vxk_head * head, const void * w, const float * x, int3
         HeadDevice scope(c.device);
         cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
         need_score_scratch(head, cs);
-        if (!head->score_logits)
-            VXK_HCUDA(cudaMalloc(&head->score_logits, (size_t) vxk::kHeadRows * c.vocab * sizeof(float)));
-        CUtensorMap map_w{};
-        encode_rows_map(&map_w, w, (int32_t) c.dtype, c.dim, c.vocab, head->tile_rows);
-        for (int32_t r0 = 0; r0 < rows; r0 += vxk::kHeadRows) {
-            vxk::HeadParams p{};
+        for (int32_t r0 = 0; r0 < rows; r0 += vxk::kScoreRows) {
+            vxk::HeadScoreParams p{};
             p.x = x + (int64_t) r0 * c.dim;
-            p.xh = head->xh;
-            p.best = head->best;
-            p.argmax = reinterpret_cast<int32_t *>(head->best);
-            p.logits = head->score_logits;
+            p.xh = head->score_xh;
+            p.part_stats = head->score_stats;
+            p.part_keys = head->score_keys;
+            p.token_logits = head->score_tokens;
+            p.row_low = head->score_low;
             p.error = head->d_error;
+            p.n_rows = std::min<int32_t>(vxk::kScoreRows, rows - r0);
             p.vocab = c.vocab;
             p.dim = c.dim;
-            p.n_rows = std::min<int32_t>(vxk::kHeadRows, rows - r0);
-            p.tile_rows = head->tile_rows;
-            p.n_tiles = head->n_tiles;
+            p.n_top = out.n_top;
             p.dtype = (int32_t) c.dtype;
-            VXK_HCUDA(vxk::launch_head(p, map_w, head->map_x, head->grid, cs));
-            vxk::ScoreLogitsParams q{};
-            q.logits = head->score_logits;
-            q.ld = c.vocab;
-            q.rows = p.n_rows;
-            q.dtype = VXK_DTYPE_F32;
-            q.parts = head->score_parts;
-            q.counters = head->score_counters;
-            q.out = out;
-            if (q.out.tokens) q.out.tokens += r0;
-            if (q.out.logprob) q.out.logprob += r0;
-            if (q.out.entropy) q.out.entropy += r0;
-            if (q.out.top_ids) q.out.top_ids += (int64_t) r0 * out.n_top;
-            if (q.out.top_logprobs) q.out.top_logprobs += (int64_t) r0 * out.n_top;
-            VXK_HCUDA(vxk::launch_score_logits(q, head->sm_count, cs));
+            const vxk::HeadScorePlan plan = vxk::head_score_plan(p.n_rows, c.vocab, head->sm_count);
+            p.n_row_tiles = plan.n_row_tiles;
+            p.tile_cols = plan.tile_cols;
+            p.n_tiles = plan.n_tiles;
+            p.n_groups = plan.n_groups;
+            p.x_box_rows = plan.x_box_rows;
+            vxk::ScoreOut o = out;
+            if (o.tokens) o.tokens += r0;
+            if (o.logprob) o.logprob += r0;
+            if (o.entropy) o.entropy += r0;
+            if (o.top_ids) o.top_ids += (int64_t) r0 * out.n_top;
+            if (o.top_logprobs) o.top_logprobs += (int64_t) r0 * out.n_top;
+            p.tokens = o.tokens;
+            CUtensorMap map_w{}, map_x{};
+            encode_rows_map(&map_w, w, (int32_t) c.dtype, c.dim, c.vocab, plan.tile_cols / plan.cg);
+            encode_rows_map(&map_x, head->score_xh, (int32_t) c.dtype, c.dim, p.n_rows, plan.x_box_rows);
+            VXK_HCUDA(vxk::launch_head_score(p, o, map_w, map_x, cs));
         }
     });
 }

@@ -285,6 +285,36 @@ struct ScoreLogitsParams {
 
 cudaError_t launch_score_logits(ScoreLogitsParams p, int sms, cudaStream_t stream);
 
+constexpr int32_t kScoreRows = 2048;  // rows of one pass over W
+
+struct HeadScorePlan {
+    int32_t cg;            // CTAs of a tile: 1 (up to 128 rows) or 2
+    int32_t n_row_tiles;   // tiles of 128 cg rows
+    int32_t tile_cols;     // vocabulary slice of a tile, a multiple of 32, <= 256
+    int32_t n_tiles;
+    int32_t n_groups;      // CTAs (pairs) that share a row tile's slices
+    int32_t x_box_rows;    // rows of x in a stage
+};
+HeadScorePlan head_score_plan(int32_t n_rows, int32_t vocab, int sms);
+
+struct HeadScoreParams {
+    const float * x;       // [n_rows][dim] fp32
+    uint16_t * xh;         // [kScoreRows][dim] in W's type
+    float4 * part_stats;   // [CTA x 2 halves][128 rows] (m, s, t, 0)
+    unsigned long long * part_keys;  // [CTA x 2 halves][n_top][128 rows]
+    float * token_logits;  // [kScoreRows]
+    uint32_t * row_low;    // [kScoreRows] value bits (top_bits) that bound the end of a row's list from below
+    const int32_t * tokens;  // [n_rows] or nullptr
+    int32_t * error;
+    int32_t n_rows, vocab, dim, n_top, dtype;
+    int32_t n_row_tiles, tile_cols, n_tiles, n_groups, x_box_rows;
+};
+
+// tmw: {dim, vocab} over W, boxes of tile_cols / cg x 64; tmx: {dim, n_rows} over xh, boxes
+// of x_box_rows x 64; both 128-byte swizzle.
+cudaError_t launch_head_score(const HeadScoreParams & p, const ScoreOut & out, const CUtensorMap & tmw,
+                              const CUtensorMap & tmx, cudaStream_t stream);
+
 // ---------------------------------------------------------------------------
 // Packed prompts (vxk_prompt_*)
 // ---------------------------------------------------------------------------

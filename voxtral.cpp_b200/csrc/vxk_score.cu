@@ -63,11 +63,12 @@ __device__ __forceinline__ uint4 load_stream(const void * p) {
 }
 
 // Strips [c0, c1) of one row by TEAM warps: adds to the thread's statistics and
-// the warp's list.  Elements before the row's first 16-byte boundary and behind
+// the warp's list.  shared_low: the largest list end of the team's warps, which no
+// warp's candidates need go below.  Elements before the row's first 16-byte boundary and behind
 // its last go with strip 0.
 template <int DT, int TEAM>
 __device__ __forceinline__ void scan(const uint8_t * row, int32_t vocab, int64_t c0, int64_t c1, int tid, Stat & a,
-                                     WarpTop & top) {
+                                     WarpTop & top, uint32_t * shared_low) {
     using E = Elem<DT>;
     constexpr int kTeam = TEAM * 32;
     const int lead = min(vocab, (int) ((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / E::kBytes);
@@ -108,9 +109,11 @@ __device__ __forceinline__ void scan(const uint8_t * row, int32_t vocab, int64_t
             for (int i = 0; i < E::kVec; ++i) m = fmaxf(m, x[j * E::kVec + i]);
         }
         if (top.n_top) {
-            // the list's end as a value: below every logit while the list is not full
-            const float low = top.low ? top_value(top.low) : -INFINITY;
-            if (__any_sync(kAll, !(m < low))) {
+            // every lane's largest element, or none where it has no element
+            const uint32_t largest = v0 < n_vec ? top_bits(m) : 0u;
+            if (top.low == 0ull) top.bound(largest);
+            if (shared_low) top.raise(*shared_low);
+            if (__any_sync(kAll, largest >= (uint32_t) (top.low >> 32))) {
 #pragma unroll
                 for (int j = 0; j < E::kLoads; ++j) {
                     const bool in = v0 + j * kTeam < n_vec;
@@ -119,6 +122,7 @@ __device__ __forceinline__ void scan(const uint8_t * row, int32_t vocab, int64_t
                     for (int i = 0; i < E::kVec; ++i)
                         top.offer(in ? top_key(x[j * E::kVec + i], idx + i) : 0ull);
                 }
+                if (shared_low && (threadIdx.x & 31) == 0) atomicMax(shared_low, (uint32_t) (top.low >> 32));
             }
         }
         if (m > a.m) stat_raise(a, m);
@@ -152,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 2) score_warp_kernel(const ScoreLogi
     top.clear(p.out.n_top);
     const int strips = p.out.vocab / (32 * kPer) + 1;
     scan<DT, 1>(static_cast<const uint8_t *>(p.logits) + row * p.ld * Elem<DT>::kBytes, p.out.vocab, 0, strips,
-                threadIdx.x & 31, a, top);
+                threadIdx.x & 31, a, top, nullptr);
     finish<DT>(p, row, warp_join(a), top.key);
 }
 
@@ -160,6 +164,7 @@ template <int DT>
 __global__ void __launch_bounds__(kThreads, 2) score_block_kernel(const ScoreLogitsParams p) {
     __shared__ Stat stats[kWarps];
     __shared__ unsigned long long lists[kWarps * kMaxTop];
+    __shared__ uint32_t shared_low;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n_top = p.out.n_top;
     const int64_t strips = p.strips, total = strips * p.rows, grid = gridDim.x, cta = blockIdx.x;
@@ -168,17 +173,20 @@ __global__ void __launch_bounds__(kThreads, 2) score_block_kernel(const ScoreLog
     for (int64_t x = begin; x < end;) {
         const int64_t row = x / strips, c0 = x - row * strips;
         const int64_t c1 = min(strips, c0 + end - x);
+        if (tid == 0) shared_low = 0;
+        __syncthreads();
         Stat a = stat_empty();
         WarpTop top;
         top.clear(n_top);
         scan<DT, kWarps>(static_cast<const uint8_t *>(p.logits) + row * p.ld * Elem<DT>::kBytes, p.out.vocab, c0, c1,
-                         tid, a, top);
+                         tid, a, top, &shared_low);
         a = warp_join(a);
         if (lane == 0) stats[warp] = a;
         if (lane < n_top) lists[warp * n_top + lane] = top.key;
         __syncthreads();
         if (warp == 0) {
             a = warp_join(lane < kWarps ? stats[lane] : stat_empty());
+            if (n_top) top.raise(shared_low);
             for (int i = n_top; i < kWarps * n_top; i += 32)  // the warp's own list is in place
                 top.offer(i + lane < kWarps * n_top ? lists[i + lane] : 0ull);
             if (c1 - c0 == strips) {
@@ -213,10 +221,16 @@ __global__ void __launch_bounds__(kThreads, 2) score_block_kernel(const ScoreLog
                         }
                         sum = stat_join(sum, warp_join(one));
                     }
-                    for (int64_t b = first; n_top && b <= last; ++b) {
+                    for (int64_t b0 = first; n_top && b0 <= last; b0 += 32) {
+                        const int64_t b = b0 + lane;
                         const bool mid = b == first && b * total / grid != r0;
                         const ScorePart * q = p.parts + 2 * b + (mid ? 1 : 0);
-                        top.offer(lane < n_top ? __ldcg(&q->top[lane]) : 0ull);
+                        for (int j = 0; j < n_top; ++j) {  // the parts' lists are in order
+                            const unsigned long long k = b <= last ? __ldcg(&q->top[j]) : 0ull;
+                            if (j == 0 && top.low == 0ull) top.bound((uint32_t) (k >> 32));
+                            if (!__any_sync(kAll, k > top.low)) break;
+                            top.offer(k);
+                        }
                     }
                     if (lane == 0) p.counters[first] = 0;
                     finish<DT>(p, row, sum, top.key);

@@ -94,11 +94,15 @@ __device__ __forceinline__ Stat stat_shfl_xor(const Stat & a, int o) {
     return {__shfl_xor_sync(kAll, a.m, o), __shfl_xor_sync(kAll, a.s, o), __shfl_xor_sync(kAll, a.t, o)};
 }
 
-__device__ __forceinline__ unsigned long long top_key(float v, int idx) {
+__device__ __forceinline__ uint32_t top_bits(float v) {
     uint32_t u = __float_as_uint(v == 0.0f ? 0.0f : v);  // -0 equals 0
     u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
     if (v != v) u = 1u;  // a NaN stands below every number (and above an empty place)
-    return ((unsigned long long) u << 32) | (unsigned long long) (0xFFFFFFFFu - (uint32_t) idx);
+    return u;
+}
+
+__device__ __forceinline__ unsigned long long top_key(float v, int idx) {
+    return ((unsigned long long) top_bits(v) << 32) | (unsigned long long) (0xFFFFFFFFu - (uint32_t) idx);
 }
 
 __device__ __forceinline__ int top_index(unsigned long long key) {
@@ -122,6 +126,25 @@ struct WarpTop {
         low = n > 0 ? 0ull : ~0ull;
         n_top = n;
     }
+    // Raises `low` before anything is listed.  Each lane holds the largest value bits
+    // (a key's upper half, 0: none) of a set of its own: the n_top-th largest of them is
+    // no more than the n_top-th largest of all elements, so nothing below it belongs to
+    // the list, and few candidates are left to insert one by one.
+    __device__ __forceinline__ void bound(uint32_t largest) {
+        const int lane = threadIdx.x & 31;
+        uint32_t v = 0;
+        for (int i = 0; i < n_top; ++i) {
+            v = __reduce_max_sync(kAll, largest);
+            if (v == 0) return;  // fewer sets than places
+            const unsigned who = __ballot_sync(kAll, largest == v);
+            if (lane == __ffs(who) - 1) largest = 0;
+        }
+        raise(v);
+    }
+    __device__ __forceinline__ void raise(uint32_t value_bits) {
+        const unsigned long long b = (unsigned long long) value_bits << 32;  // below every key of that value
+        if (n_top && b > low) low = b;
+    }
     // Inserts a key that every lane holds.
     __device__ __forceinline__ void insert(unsigned long long k) {
         const int lane = threadIdx.x & 31;
@@ -129,7 +152,8 @@ struct WarpTop {
         const unsigned long long up = __shfl_up_sync(kAll, key, 1);
         if (lane == at) key = k;
         if (lane > at) key = up;
-        low = __shfl_sync(kAll, key, n_top - 1);
+        const unsigned long long last = __shfl_sync(kAll, key, n_top - 1);
+        if (last > low) low = last;
     }
     // Offers each lane's candidate (0: none).
     __device__ __forceinline__ void offer(unsigned long long cand) {
