@@ -321,9 +321,12 @@ cudaError_t launch_head_score(const HeadScoreParams & p, const ScoreOut & out, c
 
 constexpr int32_t kErrPlan = 5;  // device error word: the plan holds more rows than the call's buffers
 
+// A plan in device memory: int4 {items, rows, sequences, byte offset of the
+// positions}, then [CTAs + 1] offsets into the items, the items of each CTA (int4
+// {first row and rows of the sequence, first token of the item, first query head}), and
+// the rows' positions.
 struct PromptRopeParams {
-    const uint8_t * plan;        // int4 {0, rows, sequences, 0} of the plan
-    const int32_t * positions;   // [rows]
+    const uint8_t * plan;
     const float2 * table;        // [max_position][head_dim / 2] (cos, sin)
     int32_t rows;                // rows of the call's buffers
     int32_t n_q, n_kv, head_dim, dtype;
@@ -338,13 +341,14 @@ struct PromptRopeParams {
 
 struct PromptAttnParams {
     const uint8_t * plan;
-    const int4 * row_seq;        // [rows] {first row of the row's sequence, its rows, 0, 0}
-    int32_t rows;
-    int32_t n_q, n_kv, head_dim, dtype;
+    int32_t off_offsets, off_items;  // byte offsets into the plan
+    int32_t rows;                // rows of the call's buffers
+    int32_t n_q, n_kv, group;    // group = n_q / n_kv
+    int32_t head_dim, dtype;
     int32_t causal, window;
+    int32_t pack_shift;          // log2 of the heads in one tile
+    int32_t tokens;              // tokens in one tile: 128 >> pack_shift
     float scale_log2;            // softmax scale * log2(e)
-    const void * q;
-    const void * k;
     const void * v;
     void * out;
     int32_t * error;
@@ -352,7 +356,10 @@ struct PromptAttnParams {
 
 cudaError_t launch_rope_table(float2 * table, int32_t rows, int32_t head_dim, double log_theta, cudaStream_t stream);
 cudaError_t launch_prompt_rope(const PromptRopeParams & p, cudaStream_t stream);
-cudaError_t launch_prompt_attention(const PromptAttnParams & p, cudaStream_t stream);
+// Tensor maps {head_dim, heads, rows} with boxes of 64 dims: tmq {64, heads of a tile,
+// tokens of a tile}, tmk and tmv {64, 1, 128}; 128-byte swizzle.
+cudaError_t launch_prompt_attention(const PromptAttnParams & p, const CUtensorMap & tmq, const CUtensorMap & tmk,
+                                    const CUtensorMap & tmv, int ctas, cudaStream_t stream);
 
 // ---------------------------------------------------------------------------
 // Quantized-weight matrix product (vxk_qweight_*)

@@ -1,5 +1,4 @@
-// Packed prompts (vxk_prompt_*): the rotary rows and the attention within each
-// sequence.
+// Rotary rows of packed prompts (vxk_prompt_rope).
 #include "vxk_internal.h"
 
 #include <cuda_bf16.h>
@@ -19,17 +18,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
-
-template <int DT>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-    if constexpr (DT == 30) {
-        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-    } else {
-        return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-    }
-}
-
-// ---- rotary rows ------------------------------------------------------------
 
 // (cos, sin) of position * theta^(-2i / head_dim), in 64 bits: at position 10^5 a
 // 32-bit angle is off by 4e-3 of a radian, more than a 16-bit value resolves.
@@ -58,7 +46,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const PromptRopeParams p) {
     if (row >= head.y) return;
     const int per_head = p.head_dim / 8;
     const int nq = p.n_q * per_head, nkv = p.n_kv * per_head;
-    const int pos = p.positions[row];
+    const int pos = reinterpret_cast<const int32_t *>(p.plan + head.w)[row];
     const float4 * turn = reinterpret_cast<const float4 *>(p.table + (int64_t) pos * (p.head_dim / 2)) +
                           (threadIdx.x % per_head) * 2;
     const float4 t0 = __ldg(turn), t1 = __ldg(turn + 1);
@@ -88,66 +76,6 @@ __global__ void __launch_bounds__(256) rope_kernel(const PromptRopeParams p) {
     }
 }
 
-// ---- attention --------------------------------------------------------------
-
-// One warp per query row and head, one key at a time: the plain form of
-//   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q . k_j,
-// with the running maximum m and sums rescaled when it grows.
-template <int DT, int HD>
-__global__ void __launch_bounds__(128) attention_kernel(const PromptAttnParams p) {
-    const int4 head = *reinterpret_cast<const int4 *>(p.plan);
-    if (head.y > p.rows) {
-        if (threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(p.error, 0, kErrPlan);
-        return;
-    }
-    constexpr int W = HD / 64;  // 32-bit words a lane holds
-    const int64_t unit = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    const int64_t row = unit / p.n_q;
-    const int h = (int) (unit - row * p.n_q);
-    if (row >= head.y) return;
-    const int4 seq = p.row_seq[row];  // first row, rows
-    const int i = (int) row - seq.x;
-    const int j0 = p.window > 0 ? max(0, i - p.window + 1) : 0;
-    const int j1 = p.causal ? i + 1 : seq.y;
-    const int hk = h / (p.n_q / p.n_kv);
-    float q[2 * W], acc[2 * W];
-    const uint32_t * qp = reinterpret_cast<const uint32_t *>(p.q) + (row * p.n_q + h) * (HD / 2) + lane * W;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        const float2 f = unpack2<DT>(qp[w]);
-        q[2 * w] = f.x * p.scale_log2;
-        q[2 * w + 1] = f.y * p.scale_log2;
-        acc[2 * w] = acc[2 * w + 1] = 0.0f;
-    }
-    float m = -INFINITY, s = 0.0f;
-    for (int j = j0; j < j1; ++j) {
-        const int64_t at = ((int64_t) (seq.x + j) * p.n_kv + hk) * (HD / 2) + lane * W;
-        float d = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float2 f = unpack2<DT>(reinterpret_cast<const uint32_t *>(p.k)[at + w]);
-            d = fmaf(q[2 * w], f.x, fmaf(q[2 * w + 1], f.y, d));
-        }
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        const float mn = fmaxf(m, d);
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float f0 = ex2(m - base), e = ex2(d - base);
-        s = s * f0 + e;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float2 f = unpack2<DT>(reinterpret_cast<const uint32_t *>(p.v)[at + w]);
-            acc[2 * w] = fmaf(acc[2 * w], f0, e * f.x);
-            acc[2 * w + 1] = fmaf(acc[2 * w + 1], f0, e * f.y);
-        }
-        m = mn;
-    }
-    uint32_t * op = reinterpret_cast<uint32_t *>(p.out) + (row * p.n_q + h) * (HD / 2) + lane * W;
-#pragma unroll
-    for (int w = 0; w < W; ++w) op[w] = pack2<DT>(acc[2 * w] / s, acc[2 * w + 1] / s);
-}
-
 }  // namespace
 
 cudaError_t launch_rope_table(float2 * table, int32_t rows, int32_t head_dim, double log_theta, cudaStream_t stream) {
@@ -161,18 +89,6 @@ cudaError_t launch_prompt_rope(const PromptRopeParams & p, cudaStream_t stream) 
         rope_kernel<30><<<(unsigned) p.rows, 256, 0, stream>>>(p);
     } else {
         rope_kernel<1><<<(unsigned) p.rows, 256, 0, stream>>>(p);
-    }
-    return cudaGetLastError();
-}
-
-cudaError_t launch_prompt_attention(const PromptAttnParams & p, cudaStream_t stream) {
-    const unsigned grid = (unsigned) (((int64_t) p.rows * p.n_q + 3) / 4);
-    if (p.head_dim == 64) {
-        if (p.dtype == 30) attention_kernel<30, 64><<<grid, 128, 0, stream>>>(p);
-        else attention_kernel<1, 64><<<grid, 128, 0, stream>>>(p);
-    } else {
-        if (p.dtype == 30) attention_kernel<30, 128><<<grid, 128, 0, stream>>>(p);
-        else attention_kernel<1, 128><<<grid, 128, 0, stream>>>(p);
     }
     return cudaGetLastError();
 }

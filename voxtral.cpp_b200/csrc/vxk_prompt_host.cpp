@@ -4,12 +4,14 @@
 #include "vxk_internal.h"
 
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <chrono>
 #include <cmath>
 #include <cstring>
 #include <new>
+#include <queue>
 #include <string>
 #include <thread>
 #include <vector>
@@ -52,6 +54,33 @@ private:
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
+constexpr size_t kPlanHead = 16;
+constexpr int32_t kKeyTile = 128;
+
+// Tensor map {head_dim, heads, rows} over packed 16-bit rows, boxes of 64 dims x
+// box_heads x box_rows, 128-byte swizzle, zero fill behind the last row.
+void encode_heads_map(CUtensorMap * map, const void * base, const vxk_prompt_config & c, int32_t heads, int64_t rows,
+                      int32_t box_heads, int32_t box_rows) {
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    if (!encode) {
+        void * fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess || !fn)
+            pfail(VXK_STATUS_BACKEND_ERROR, "cuTensorMapEncodeTiled is not available");
+        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }
+    const cuuint64_t dims[3] = {(cuuint64_t) c.head_dim, (cuuint64_t) heads, (cuuint64_t) rows};
+    const cuuint64_t strides[2] = {(cuuint64_t) c.head_dim * 2, (cuuint64_t) c.head_dim * 2 * (cuuint64_t) heads};
+    const cuuint32_t box[3] = {64, (cuuint32_t) box_heads, (cuuint32_t) box_rows};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    const CUresult r = encode(map, c.dtype == VXK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                              3, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) pfail(VXK_STATUS_BACKEND_ERROR, "cuTensorMapEncodeTiled failed for a packed prompt");
+}
+
 }  // namespace
 
 struct vxk_prompt {
@@ -62,8 +91,9 @@ struct vxk_prompt {
     cudaEvent_t plan_ev[2] = {nullptr, nullptr};
     int plan_next = 0;
     size_t plan_bytes = 0;
-    size_t off_positions = 0;   // offsets into the plan
-    size_t off_row_seq = 0;
+    size_t off_items = 0;       // offsets into the plan; CTA offsets follow its head
+    int32_t pack_shift = 0;     // log2 of the query heads in one tile
+    int32_t tokens = 0;         // tokens in one tile
     int32_t * d_error = nullptr;
     cudaEvent_t ev_sync = nullptr;
     int sm_count = 0;
@@ -178,9 +208,14 @@ vxk_status vxk_prompt_create(const vxk_prompt_config * config, vxk_prompt ** out
         }
         PromptDevice scope(c.device);
         VXK_PCUDA(cudaDeviceGetAttribute(&p->sm_count, cudaDevAttrMultiProcessorCount, c.device));
-        p->off_positions = 16;
-        p->off_row_seq = p->off_positions + align16((size_t) c.max_rows * sizeof(int32_t));
-        p->plan_bytes = p->off_row_seq + (size_t) c.max_rows * sizeof(int4);
+        const int32_t group = c.n_q_heads / c.n_kv_heads;
+        while (p->pack_shift < 7 && group % (2 << p->pack_shift) == 0) ++p->pack_shift;
+        p->tokens = 128 >> p->pack_shift;
+        // a sequence's last item may be a part of one
+        const size_t max_items = ((size_t) c.max_rows / (2 * p->tokens) + (size_t) std::min(c.max_seqs, c.max_rows)) *
+                                 (size_t) (c.n_q_heads >> p->pack_shift);
+        p->off_items = kPlanHead + align16((size_t) (p->sm_count + 1) * sizeof(int32_t));
+        p->plan_bytes = p->off_items + max_items * sizeof(int4) + (size_t) c.max_rows * sizeof(int32_t);
         VXK_PCUDA(cudaMalloc(&p->d_plan, p->plan_bytes));
         for (int i = 0; i < 2; ++i) {
             VXK_PCUDA(cudaHostAlloc(reinterpret_cast<void **>(&p->h_plan[i]), p->plan_bytes, cudaHostAllocDefault));
@@ -238,19 +273,52 @@ vxk_status vxk_prompt_plan(vxk_prompt * prompt, const int32_t * n_rows, const in
         const int slot = prompt->plan_next;
         VXK_PCUDA(cudaEventSynchronize(prompt->plan_ev[slot]));
         uint8_t * h = prompt->h_plan[slot];
-        const int32_t head[4] = {0, (int32_t) total, n_seqs, 0};
-        std::memcpy(h, head, sizeof(head));
-        int32_t * pos = reinterpret_cast<int32_t *>(h + prompt->off_positions);
-        int4 * seq = reinterpret_cast<int4 *>(h + prompt->off_row_seq);
-        int32_t row = 0;
-        for (int32_t i = 0; i < n_seqs; ++i) {
-            const int32_t row0 = row;
-            for (int32_t j = 0; j < n_rows[i]; ++j, ++row) {
-                pos[row] = (first_position ? first_position[i] : 0) + j;
-                seq[row] = make_int4(row0, n_rows[i], 0, 0);
+
+        // Items with their cost (key tiles, and about two for filling and emptying the
+        // pipeline), longest first, each to the CTA with the least work so far.
+        struct Work {
+            int32_t cost;
+            int4 item;
+        };
+        std::vector<Work> work;
+        const int32_t per_item = 2 * prompt->tokens, pack = 1 << prompt->pack_shift;
+        int32_t row0 = 0;
+        for (int32_t i = 0; i < n_seqs; row0 += n_rows[i], ++i) {
+            for (int32_t t0 = 0; t0 < n_rows[i]; t0 += per_item) {
+                const int32_t last = c.causal ? std::min(t0 + per_item, n_rows[i]) - 1 : n_rows[i] - 1;
+                const int32_t lo = c.window > 0 ? std::max(0, t0 - c.window + 1) / kKeyTile : 0;
+                for (int32_t hq = 0; hq < c.n_q_heads; hq += pack)
+                    work.push_back({last / kKeyTile + 1 - lo + 2, make_int4(row0, n_rows[i], t0, hq)});
             }
         }
-        VXK_PCUDA(cudaMemcpyAsync(prompt->d_plan, h, prompt->plan_bytes, cudaMemcpyHostToDevice, cs));
+        std::stable_sort(work.begin(), work.end(), [](const Work & a, const Work & b) { return a.cost > b.cost; });
+        std::vector<std::vector<int32_t>> mine((size_t) prompt->sm_count);
+        using Load = std::pair<int64_t, int32_t>;
+        std::priority_queue<Load, std::vector<Load>, std::greater<Load>> load;
+        for (int32_t i = 0; i < prompt->sm_count; ++i) load.push({0, i});
+        for (size_t w = 0; w < work.size(); ++w) {
+            const Load l = load.top();
+            load.pop();
+            mine[(size_t) l.second].push_back((int32_t) w);
+            load.push({l.first + work[w].cost, l.second});
+        }
+        int32_t * offsets = reinterpret_cast<int32_t *>(h + kPlanHead);
+        int4 * items = reinterpret_cast<int4 *>(h + prompt->off_items);
+        int32_t at = 0;
+        for (int32_t i = 0; i < prompt->sm_count; ++i) {
+            offsets[i] = at;
+            for (const int32_t w : mine[(size_t) i]) items[at++] = work[(size_t) w].item;
+        }
+        offsets[prompt->sm_count] = at;
+        const size_t off_positions = prompt->off_items + (size_t) at * sizeof(int4);
+        int32_t * pos = reinterpret_cast<int32_t *>(h + off_positions);
+        for (int32_t i = 0; i < n_seqs; ++i)
+            for (int32_t j = 0; j < n_rows[i]; ++j) *pos++ = (first_position ? first_position[i] : 0) + j;
+        if (off_positions > (size_t) INT32_MAX) pfail(VXK_STATUS_INVALID_ARGUMENT, "the plan is too large");
+        const int32_t head[4] = {at, (int32_t) total, n_seqs, (int32_t) off_positions};
+        std::memcpy(h, head, sizeof(head));
+        VXK_PCUDA(cudaMemcpyAsync(prompt->d_plan, h, off_positions + (size_t) total * sizeof(int32_t),
+                                  cudaMemcpyHostToDevice, cs));
         VXK_PCUDA(cudaEventRecord(prompt->plan_ev[slot], cs));
         prompt->plan_next ^= 1;
         prompt->rows = (int32_t) total;
@@ -275,7 +343,6 @@ vxk_status vxk_prompt_rope(vxk_prompt * prompt, const float * q, const float * k
         PromptDevice scope(c.device);
         vxk::PromptRopeParams a{};
         a.plan = prompt->d_plan;
-        a.positions = reinterpret_cast<const int32_t *>(prompt->d_plan + prompt->off_positions);
         a.table = prompt->table;
         a.rows = prompt->rows;
         a.n_q = c.n_q_heads;
@@ -303,22 +370,28 @@ vxk_status vxk_prompt_attention(vxk_prompt * prompt, const void * q, const void 
         PromptDevice scope(c.device);
         vxk::PromptAttnParams a{};
         a.plan = prompt->d_plan;
-        a.row_seq = reinterpret_cast<const int4 *>(prompt->d_plan + prompt->off_row_seq);
+        a.off_offsets = (int32_t) kPlanHead;
+        a.off_items = (int32_t) prompt->off_items;
         a.rows = prompt->rows;
         a.n_q = c.n_q_heads;
         a.n_kv = c.n_kv_heads;
+        a.group = c.n_q_heads / c.n_kv_heads;
+        a.pack_shift = prompt->pack_shift;
+        a.tokens = prompt->tokens;
         a.head_dim = c.head_dim;
         a.dtype = (int32_t) c.dtype;
         a.causal = c.causal;
         a.window = c.window;
         const double scale = c.scale > 0.0f ? (double) c.scale : 1.0 / std::sqrt((double) c.head_dim);
         a.scale_log2 = (float) (scale * 1.4426950408889634);
-        a.q = q;
-        a.k = k;
         a.v = v;
         a.out = out;
         a.error = prompt->d_error;
-        VXK_PCUDA(vxk::launch_prompt_attention(a, static_cast<cudaStream_t>(cuda_stream)));
+        CUtensorMap mq{}, mk{}, mv{};
+        encode_heads_map(&mq, q, c, c.n_q_heads, prompt->rows, 1 << prompt->pack_shift, prompt->tokens);
+        encode_heads_map(&mk, k, c, c.n_kv_heads, prompt->rows, 1, kKeyTile);
+        encode_heads_map(&mv, v, c, c.n_kv_heads, prompt->rows, 1, kKeyTile);
+        VXK_PCUDA(vxk::launch_prompt_attention(a, mq, mk, mv, prompt->sm_count, static_cast<cudaStream_t>(cuda_stream)));
     });
 }
 
