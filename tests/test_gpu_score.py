@@ -351,3 +351,31 @@ def test_hidden_rows_same_every_time_and_inside_a_graph(vxk):
         assert all(torch.equal(a, b) for a, b in zip(outs, first))
     head.sync(_stream())
     head.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_lists_of_rising_falling_and_equal_logits(vxk, dtype):
+    """Rows whose every strip beats the last (or ties with it), and strips full of candidates."""
+    import torch
+
+    vocab, n_top = 70001, 16
+    i = torch.arange(vocab, device="cuda", dtype=torch.float32)
+    l = torch.stack([i / 64, -i / 64, torch.zeros_like(i), torch.floor(i / 5000), -torch.floor(i / 5000),
+                     torch.where(i % 4096 < 3000, i, -i) / 128, (i % 7 == 3).float(),
+                     torch.where(i > 60000, torch.full_like(i, 5.0), i * 0)]).to(_torch_type(dtype))
+    tokens = np.arange(8) * 7000
+    check(score_logits(vxk, l, vocab, tokens, n_top), l.double().cpu().numpy(), tokens, n_top)
+
+
+def test_hidden_rows_with_equal_logits(vxk):
+    """Zero rows make every logit 0: the lowest indices are listed and the distribution is even."""
+    import torch
+
+    vocab, dim, rows = 9001, 128, 140
+    w = torch.randn(vocab, dim, device="cuda").half()
+    x = torch.randn(rows, dim, device="cuda")
+    x[::3] = 0.0
+    for n_top in (1, 4, 16):
+        lp, ent, ids, top = run_head(vxk, w, x, np.arange(rows), n_top, F16)
+        assert np.array_equal(ids[::3], np.tile(np.arange(n_top), (len(ids[::3]), 1)))
+        assert np.allclose(lp[::3], -np.log(vocab), rtol=1e-6) and np.allclose(ent[::3], np.log(vocab), rtol=1e-6)

@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                 if (tile == group) bound = __ldcg(&p.row_low[row]);  // the others' first bounds, as they come
                 if ((unsigned long long) bound << 32 > low_key) {
                     low_key = (unsigned long long) bound << 32;
-                    low = top_value(low_key - 1);  // the next value below
+                    low = top_below(bound);
                 }
                 if (!(m <= low)) {
                     const unsigned long long before = low_key;

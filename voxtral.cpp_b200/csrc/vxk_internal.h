@@ -270,7 +270,7 @@ cudaError_t launch_head_argmax(const float * logits, int32_t rows, int32_t vocab
 // Scores of rows of logits (vxk_head_score_logits, vxk_head_score)
 // ---------------------------------------------------------------------------
 
-constexpr int kScoreCtasPerSm = 2;  // CTAs of the logits kernel per multiprocessor
+constexpr int kScoreCtasPerSm = 3;  // CTAs of the logits kernel per multiprocessor
 
 struct ScoreLogitsParams {
     const void * logits;   // [rows][ld] of dtype

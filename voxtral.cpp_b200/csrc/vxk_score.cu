@@ -2,20 +2,27 @@
 // log probability, entropy and top list in one pass (the mathematics is in
 // vxk_score.h).  Bound by reading the logits once.
 //
-// The rows' elements are cut into strips of 4096; a CTA takes an equal, unbroken
-// run of all rows' strips, so that any number of rows keeps the whole device busy
-// to the end: a row that lies within one CTA's run is finished there, one that
-// crosses into others' leaves a part in each, and the CTA that arrives last joins
-// them in order (the result does not depend on which that is).  Rows of at most
-// one strip go one to a warp instead: there the block's reductions would cost more
-// than the read.
+// The rows' elements are cut into strips of 4096; a CTA takes an equal, unbroken run of
+// all rows' strips, so that any number of rows keeps the whole device busy to the end: a
+// row that lies within one CTA's run is finished there, one that crosses into others'
+// leaves a part in each, and the CTA that arrives last joins them (the result does not
+// depend on which that is).  Rows of at most one strip go one to a warp instead: there the
+// block's reductions would cost more than the read.
 //
-// A thread holds 16 elements of a strip at a time (16-byte loads), takes their
-// maximum first, so that the sums are rescaled at most once a strip, and offers
-// candidates to its warp's top list only where that maximum reaches the list's
-// end.
+// Strips reach shared memory by bulk copies, two ahead of the one that is read.  A thread
+// takes 16 elements of each and their maximum first, so that the sums are rescaled at
+// most once a strip.
+//
+// The top list is found by comparing with a lower bound of its end and collecting the few
+// keys that reach it in shared memory.  In a run's first strip every warp takes the
+// n_top-th largest of its lanes' maxima, which is no more than the n_top-th largest of
+// all; after that strip, the fourth and every sixteenth (t strips bring about n_top keys
+// above the bound of the t before them) the keys are ranked against each other, all at
+// once, and the list's end becomes the bound.  Keys that do not fit (equal or rising logits) send their strips
+// through a slower bound of which at most n_top groups of 64 elements can be above.
 #include "vxk_internal.h"
 #include "vxk_score.h"
+#include "vxk_tc.h"
 
 #include <algorithm>
 
@@ -24,13 +31,14 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPer = 16;  // elements of a strip in one thread
+constexpr int kRowOfWarp = 4096;  // a row of at most so many elements is one warp's
 
 template <int DT>
 struct Elem {
     static constexpr int kBytes = DT == 0 ? 4 : 2;
     static constexpr int kVec = 16 / kBytes;      // elements of a 16-byte load
-    static constexpr int kLoads = kPer / kVec;    // loads of a strip in one thread
+    static constexpr int kPer = 16;               // elements of a strip in one thread
+    static constexpr int kLoads = kPer / kVec;    // their vectors
 };
 
 template <int DT>
@@ -62,74 +70,62 @@ __device__ __forceinline__ uint4 load_stream(const void * p) {
     return u;
 }
 
-// Strips [c0, c1) of one row by TEAM warps: adds to the thread's statistics and
-// the warp's list.  shared_low: the largest list end of the team's warps, which no
-// warp's candidates need go below.  Elements before the row's first 16-byte boundary and behind
-// its last go with strip 0.
-template <int DT, int TEAM>
-__device__ __forceinline__ void scan(const uint8_t * row, int32_t vocab, int64_t c0, int64_t c1, int tid, Stat & a,
-                                     WarpTop & top, uint32_t * shared_low) {
-    using E = Elem<DT>;
-    constexpr int kTeam = TEAM * 32;
-    const int lead = min(vocab, (int) ((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / E::kBytes);
-    const int n_vec = (vocab - lead) / E::kVec;
-    const uint8_t * body = row + (int64_t) lead * E::kBytes;
+// A row in memory: elements before its first 16-byte boundary, whole 16-byte vectors, and
+// those behind the last.
+template <int DT>
+struct Row {
+    const uint8_t * at;
+    const uint8_t * body;
+    int vocab, lead, n_vec;
+    __device__ __forceinline__ Row(const ScoreLogitsParams & p, int64_t row) {
+        using E = Elem<DT>;
+        at = static_cast<const uint8_t *>(p.logits) + row * p.ld * E::kBytes;
+        vocab = p.out.vocab;
+        lead = min(vocab, (int) ((16 - (reinterpret_cast<uintptr_t>(at) & 15)) & 15) / E::kBytes);
+        n_vec = (vocab - lead) / E::kVec;
+        body = at + (int64_t) lead * E::kBytes;
+    }
+    // Thread t's element of those outside the vectors, -1: none (t < 32 suffices).
+    __device__ __forceinline__ int ragged(int t) const {
+        const int tail = lead + n_vec * Elem<DT>::kVec;
+        if (t < lead) return t;
+        return t >= 16 && t - 16 < vocab - tail ? tail + t - 16 : -1;
+    }
+};
 
-    if (c0 == 0) {
-        const int tail0 = lead + n_vec * E::kVec;
-        int idx = -1;
-        if (tid < lead) idx = tid;
-        else if (tid >= 16 && tid - 16 < vocab - tail0) idx = tail0 + tid - 16;
-        if (__any_sync(kAll, idx >= 0)) {
-            const float v = idx >= 0 ? logit_at<DT>(row, idx) : -INFINITY;
-            const float m = fmaxf(a.m, v);
-            stat_raise(a, m);
-            if (idx >= 0) stat_add(a, v, stat_base(m));
-            if (top.n_top) top.offer(idx >= 0 ? top_key(v, idx) : 0ull);
+// A thread's elements of a strip whose vectors start at v0, `team` apart, from where they
+// lie (global memory, or the strip's copy in shared memory); -inf where there is none.
+// Returns the largest.
+template <int DT, bool SHARED>
+__device__ __forceinline__ float take_strip(const Row<DT> & r, const uint8_t * from, int v0, int team,
+                                            float (&x)[Elem<DT>::kPer]) {
+    using E = Elem<DT>;
+    uint4 u[E::kLoads];
+#pragma unroll
+    for (int j = 0; j < E::kLoads; ++j)
+        if (v0 + j * team < r.n_vec)
+            u[j] = SHARED ? *reinterpret_cast<const uint4 *>(from + j * team * 16) : load_stream(from + (int64_t) j * team * 16);
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < E::kLoads; ++j) {
+        if (v0 + j * team < r.n_vec) {
+            unpack<DT>(u[j], x + j * E::kVec);
+        } else {
+#pragma unroll
+            for (int i = 0; i < E::kVec; ++i) x[j * E::kVec + i] = -INFINITY;
         }
+#pragma unroll
+        for (int i = 0; i < E::kVec; ++i) m = fmaxf(m, x[j * E::kVec + i]);
     }
-    for (int64_t c = c0; c < c1; ++c) {
-        const int64_t v0 = c * (kTeam * E::kLoads) + tid;
-        if (c * (kTeam * E::kLoads) >= n_vec) break;
-        float x[kPer];
-        uint4 u[E::kLoads];
+    return m;
+}
+
+template <int N>
+__device__ __forceinline__ void add_strip(Stat & a, const float (&x)[N], float m) {
+    if (m > a.m) stat_raise(a, m);
+    const float base = stat_base(a.m);
 #pragma unroll
-        for (int j = 0; j < E::kLoads; ++j)
-            if (v0 + j * kTeam < n_vec) u[j] = load_stream(body + (v0 + j * kTeam) * 16);
-        float m = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < E::kLoads; ++j) {
-            if (v0 + j * kTeam < n_vec) {
-                unpack<DT>(u[j], x + j * E::kVec);
-            } else {
-#pragma unroll
-                for (int i = 0; i < E::kVec; ++i) x[j * E::kVec + i] = -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < E::kVec; ++i) m = fmaxf(m, x[j * E::kVec + i]);
-        }
-        if (top.n_top) {
-            // every lane's largest element, or none where it has no element
-            const uint32_t largest = v0 < n_vec ? top_bits(m) : 0u;
-            if (top.low == 0ull) top.bound(largest);
-            if (shared_low) top.raise(*shared_low);
-            if (__any_sync(kAll, largest >= (uint32_t) (top.low >> 32))) {
-#pragma unroll
-                for (int j = 0; j < E::kLoads; ++j) {
-                    const bool in = v0 + j * kTeam < n_vec;
-                    const int idx = lead + (int) (v0 + j * kTeam) * E::kVec;
-#pragma unroll
-                    for (int i = 0; i < E::kVec; ++i)
-                        top.offer(in ? top_key(x[j * E::kVec + i], idx + i) : 0ull);
-                }
-                if (shared_low && (threadIdx.x & 31) == 0) atomicMax(shared_low, (uint32_t) (top.low >> 32));
-            }
-        }
-        if (m > a.m) stat_raise(a, m);
-        const float base = stat_base(a.m);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) stat_add(a, x[i], base);
-    }
+    for (int i = 0; i < N; ++i) stat_add(a, x[i], base);
 }
 
 __device__ __forceinline__ Stat warp_join(Stat a) {
@@ -147,111 +143,395 @@ __device__ __forceinline__ void finish(const ScoreLogitsParams & p, int64_t row,
     score_write(p.out, row, a, key, token, l);
 }
 
+// A row of at most one strip by one warp, its list in the warp's lanes.
 template <int DT>
 __global__ void __launch_bounds__(kThreads, 2) score_warp_kernel(const ScoreLogitsParams p) {
+    using E = Elem<DT>;
     const int64_t row = (int64_t) blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
     if (row >= p.rows) return;
+    const Row<DT> r(p, row);
     Stat a = stat_empty();
     WarpTop top;
     top.clear(p.out.n_top);
-    const int strips = p.out.vocab / (32 * kPer) + 1;
-    scan<DT, 1>(static_cast<const uint8_t *>(p.logits) + row * p.ld * Elem<DT>::kBytes, p.out.vocab, 0, strips,
-                threadIdx.x & 31, a, top, nullptr);
+    const int idx = r.ragged(lane);
+    if (idx >= 0) {
+        const float v = logit_at<DT>(r.at, idx);
+        stat_raise(a, v > a.m ? v : a.m);
+        stat_add(a, v, stat_base(a.m));
+    }
+    if (top.n_top) top.offer(idx >= 0 ? top_key(logit_at<DT>(r.at, idx), idx) : 0ull);
+    for (int first = 0; first < r.n_vec; first += 32 * E::kLoads) {
+        const int v0 = first + lane;
+        float x[E::kPer];
+        const float m = take_strip<DT, false>(r, r.body + (int64_t) v0 * 16, v0, 32, x);
+        if (top.n_top) {
+            // every lane's largest element, or none where it has no element
+            const uint32_t largest = v0 < r.n_vec ? top_bits(m) : 0u;
+            if (top.low == 0ull) top.bound(largest);
+            if (__any_sync(kAll, largest >= (uint32_t) (top.low >> 32))) {
+#pragma unroll
+                for (int j = 0; j < E::kLoads; ++j) {
+                    const bool in = v0 + j * 32 < r.n_vec;
+                    const int at = r.lead + (int) (v0 + j * 32) * E::kVec;
+#pragma unroll
+                    for (int i = 0; i < E::kVec; ++i) top.offer(in ? top_key(x[j * E::kVec + i], at + i) : 0ull);
+                }
+            }
+        }
+        add_strip(a, x, m);
+    }
     finish<DT>(p, row, warp_join(a), top.key);
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads, 2) score_block_kernel(const ScoreLogitsParams p) {
-    __shared__ Stat stats[kWarps];
-    __shared__ unsigned long long lists[kWarps * kMaxTop];
-    __shared__ uint32_t shared_low;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int n_top = p.out.n_top;
-    const int64_t strips = p.strips, total = strips * p.rows, grid = gridDim.x, cta = blockIdx.x;
-    const int64_t begin = cta * total / grid, end = (cta + 1) * total / grid;
+constexpr int kKeys = 2304;    // collected keys of a run: 8 warps x 16 lanes x 16, and ragged ends
+constexpr int kStages = 4;     // strips of a CTA under way or being read
+// The list's code needs more registers than three CTAs of an SM leave.
+constexpr int ctas_per_sm(bool list) { return list ? 2 : kScoreCtasPerSm; }
+constexpr int kSpare = 8;      // keys beyond n_top that are let be
+constexpr int kLook = 16;      // most strips between two looks at their number
 
-    for (int64_t x = begin; x < end;) {
-        const int64_t row = x / strips, c0 = x - row * strips;
-        const int64_t c1 = min(strips, c0 + end - x);
-        if (tid == 0) shared_low = 0;
-        __syncthreads();
+struct Collected {
+    unsigned long long key[kKeys];
+    unsigned long long best[kMaxTop];
+    unsigned long long group[kThreads];
+    unsigned long long bound;  // a key that bounds the list's end from below
+    uint32_t warm;             // the upper half of one (any key of that value may belong to the list)
+    int count;
+};
+
+// Ranks `n` collected keys (all threads; n is the same for all): the n_top largest, in
+// order, stay, and the list's end becomes the bound.
+__device__ __forceinline__ void rank_keys(Collected & c, int n, int n_top) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const unsigned long long mine = c.key[i];
+        int above = 0;
+        for (int j = 0; j < n; ++j) above += c.key[j] > mine;
+        if (above < n_top) c.best[above] = mine;
+    }
+    __syncthreads();
+    if ((int) threadIdx.x < n_top) c.key[threadIdx.x] = (int) threadIdx.x < n ? c.best[threadIdx.x] : 0ull;
+    if (threadIdx.x == 0) {
+        c.count = min(n, n_top);
+        if (n >= n_top) c.bound = max(c.bound, c.best[n_top - 1]);
+    }
+    __syncthreads();
+}
+
+// The same for all that were collected, as all threads see them behind a barrier.
+__device__ __forceinline__ void rank_kept(Collected & c, int n_top) {
+    const int n = c.count;
+    __syncthreads();
+    rank_keys(c, n, n_top);
+}
+
+// What the bound leaves in question is above this.
+__device__ __forceinline__ float below_bound(const Collected & c) {
+    return top_below(max((uint32_t) (c.bound >> 32), c.warm));
+}
+
+// Appends a thread's keys of a strip that reach the bound (low: below_bound, or an older
+// one's); returns whether many are there.
+template <int DT>
+__device__ __forceinline__ bool collect(Collected & c, const Row<DT> & r, int v0, const float (&x)[Elem<DT>::kPer],
+                                        float m, float low, int n_top) {
+    using E = Elem<DT>;
+    if (v0 >= r.n_vec || m <= low) return false;
+    const unsigned long long bound = max(c.bound, (unsigned long long) c.warm << 32);
+    bool many = false;
+#pragma unroll
+    for (int j = 0; j < E::kLoads; ++j) {
+        if (v0 + j * kThreads >= r.n_vec) break;
+#pragma unroll
+        for (int i = 0; i < E::kVec; ++i) {
+            const float v = x[j * E::kVec + i];
+            if (!(v <= low)) {
+                const unsigned long long k = top_key(v, r.lead + (v0 + j * kThreads) * E::kVec + i);
+                if (k >= bound) {
+                    const int place = atomicAdd(&c.count, 1);
+                    if (place < kKeys) c.key[place] = k;
+                    many |= place >= n_top + kSpare;
+                }
+            }
+        }
+    }
+    return many;
+}
+
+// A strip whose keys may not fit: its own bound first, then its keys, behind the `before`
+// keys of earlier strips (the same number in all threads).
+template <int DT>
+__device__ __forceinline__ void collect_first(Collected & c, const Row<DT> & r, int v0, const float (&x)[Elem<DT>::kPer],
+                                              float m, int before, int n_top) {
+    using E = Elem<DT>;
+    int at = -1;  // the lowest index of the thread's largest element
+#pragma unroll
+    for (int j = E::kLoads - 1; j >= 0; --j)
+#pragma unroll
+        for (int i = E::kVec - 1; i >= 0; --i)
+            if (v0 + j * kThreads < r.n_vec && top_bits(x[j * E::kVec + i]) == top_bits(m))
+                at = r.lead + (int) (v0 + j * kThreads) * E::kVec + i;
+    const unsigned long long mine = v0 < r.n_vec ? top_key(m, at) : 0ull;
+    unsigned long long g = max(mine, __shfl_xor_sync(kAll, mine, 1));
+    g = max(g, __shfl_xor_sync(kAll, g, 2));
+    if (threadIdx.x % 4 == 0) c.group[threadIdx.x / 4] = g;
+    __syncthreads();
+    if (threadIdx.x < kThreads / 4) {
+        const unsigned long long k = c.group[threadIdx.x];
+        int above = 0;
+        for (int j = 0; j < kThreads / 4; ++j) above += c.group[j] > k;
+        if (above == n_top - 1 && k > c.bound) c.bound = k;  // keys differ: one thread
+    }
+    if (threadIdx.x == 0) c.count = before;
+    __syncthreads();
+    collect(c, r, v0, x, m, below_bound(c), n_top);
+    __syncthreads();
+}
+
+template <int DT, bool LIST>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(LIST)) score_block_kernel(const ScoreLogitsParams p) {
+    using E = Elem<DT>;
+    __shared__ Stat stats[kWarps];
+    __shared__ Collected keys;
+    __shared__ int arrived;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n_top = LIST ? p.out.n_top : 0;
+    const int strips = (int) p.strips;
+    const int64_t total = strips * p.rows;
+    const uint32_t grid = gridDim.x, cta = blockIdx.x;
+    const int64_t begin = cta * total / grid, end = (cta + 1) * total / grid;
+    constexpr int kStep = kThreads * E::kLoads;  // vectors of a strip
+    constexpr int kStripBytes = kStep * 16;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ uint64_t full[kStages], empty[kStages];
+    __shared__ volatile int32_t abort_flag;
+
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kWarps);
+        }
+        abort_flag = 0;
+        mbar_fence_init();
+    }
+    __syncthreads();
+    // Strips under way: thread 0 copies the run's next strip as soon as the warps have read
+    // the one in its place.  A wait that runs out sets the error word and goes on: what
+    // is then read is wrong but lies in the ring.
+    __shared__ int64_t fed_row;  // thread 0's: the strip to copy next
+    __shared__ int fed_strip;
+    if (tid == 0) {
+        fed_row = begin / strips;
+        fed_strip = (int) (begin % strips);
+    }
+    uint32_t turn = 0;
+    auto feed = [&](uint32_t nth) {  // the run's nth strip
+        if (tid != 0 || (int64_t) nth >= end - begin) return;
+        const int st = nth % kStages;
+        tc_wait(&empty[st], ((nth / kStages) & 1) ^ 1, &abort_flag, p.out.error);
+        const Row<DT> r(p, fed_row);
+        const int v0 = fed_strip * kStep;
+        const uint32_t bytes = (uint32_t) max(0, min(kStep, r.n_vec - v0)) * 16;
+        mbar_expect_tx(&full[st], bytes);
+        if (bytes) bulk_load(ring + st * kStripBytes, r.body + (int64_t) v0 * 16, bytes, &full[st]);
+        if (++fed_strip == strips) {
+            fed_strip = 0;
+            ++fed_row;
+        }
+    };
+    for (int i = 0; i < kStages - 1; ++i) feed(i);
+
+    for (int64_t at = begin; at < end;) {
+        const int64_t row = at / strips;
+        const int c0 = (int) (at - row * strips), c1 = (int) min((int64_t) strips, c0 + end - at);
+        const Row<DT> r(p, row);
         Stat a = stat_empty();
-        WarpTop top;
-        top.clear(n_top);
-        scan<DT, kWarps>(static_cast<const uint8_t *>(p.logits) + row * p.ld * Elem<DT>::kBytes, p.out.vocab, c0, c1,
-                         tid, a, top, &shared_low);
+        if (tid == 0) {
+            keys.bound = 0ull;
+            keys.warm = 0u;
+            keys.count = 0;
+        }
+        __syncthreads();
+        if (c0 == 0) {
+            const int idx = r.ragged(tid);
+            if (idx >= 0) {
+                const float v = logit_at<DT>(r.at, idx);
+                stat_raise(a, v > a.m ? v : a.m);
+                stat_add(a, v, stat_base(a.m));
+                if (n_top) keys.key[atomicAdd(&keys.count, 1)] = top_key(v, idx);
+            }
+            __syncthreads();
+        }
+        const int ragged = keys.count;
+        __syncthreads();
+        bool many = false;
+        float low = __uint_as_float(0x7fc00000u);
+        int since = c0;                  // first strip since the last look
+        for (int c = c0; c < c1; ++c) {
+            const int v0 = c * kStep + tid;
+            float x[E::kPer];
+            const int st = turn % kStages;
+            tc_wait(&full[st], (turn / kStages) & 1, &abort_flag, p.out.error);
+            const float m = take_strip<DT, true>(r, ring + st * kStripBytes + tid * 16, v0, kThreads, x);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+            ++turn;
+            feed(turn + kStages - 2);
+            add_strip(a, x, m);
+            if constexpr (LIST) {
+                if (c == c0) {
+                    // the n_top-th largest of the lanes' maxima
+                    uint32_t largest = v0 < r.n_vec ? top_bits(m) : 0u, v = 0;
+                    for (int i = 0; i < n_top; ++i) {
+                        v = __reduce_max_sync(kAll, largest);
+                        const unsigned who = __ballot_sync(kAll, largest == v);
+                        if (lane == __ffs(who) - 1) largest = 0u;
+                    }
+                    if (lane == 0) atomicMax(&keys.warm, v);  // 0: fewer lanes than places
+                    __syncwarp();
+                    low = below_bound(keys);
+                }
+                many |= collect(keys, r, v0, x, m, low, n_top);
+                const int seen = c - c0 + 1;
+                if (seen == 1 || seen == 4 || seen % kLook == 0 || c + 1 == c1) {
+                    if (__syncthreads_or(many)) {
+                        many = false;
+                        if (keys.count > kKeys) {
+                            // they did not fit: back to those of the strips before the last look
+                            // (at most n_top + kSpare, or they would have been ranked), then the
+                            // strips since, one by one
+                            __syncthreads();
+                            if (tid == 0) {
+                                const int64_t lo = r.lead + (int64_t) since * kStep * E::kVec;
+                                const int64_t hi =
+                                    r.lead + min((int64_t) (c + 1) * kStep, (int64_t) r.n_vec) * E::kVec;
+                                int n = 0;
+                                for (int i = 0; i < max(n_top + kSpare, ragged); ++i) {
+                                    const unsigned long long k = keys.key[i];
+                                    if (top_index(k) < lo || top_index(k) >= hi) keys.key[n++] = k;
+                                }
+                                keys.count = n;
+                            }
+                            __syncthreads();
+                            for (int again = since; again <= c; ++again) {
+                                const int before = keys.count;
+                                __syncthreads();
+                                const int w0 = again * kStep + tid;
+                                const float most =
+                                    take_strip<DT, false>(r, r.body + (int64_t) w0 * 16, w0, kThreads, x);
+                                collect_first(keys, r, w0, x, most, before, n_top);
+                                rank_kept(keys, n_top);
+                            }
+                        } else {
+                            rank_kept(keys, n_top);
+                        }
+                    }
+                    since = c + 1;
+                    low = below_bound(keys);
+                }
+            }
+        }
         a = warp_join(a);
         if (lane == 0) stats[warp] = a;
-        if (lane < n_top) lists[warp * n_top + lane] = top.key;
         __syncthreads();
+        if (n_top) {
+            rank_kept(keys, n_top);
+        }
         if (warp == 0) {
-            a = warp_join(lane < kWarps ? stats[lane] : stat_empty());
-            if (n_top) top.raise(shared_low);
-            for (int i = n_top; i < kWarps * n_top; i += 32)  // the warp's own list is in place
-                top.offer(i + lane < kWarps * n_top ? lists[i + lane] : 0ull);
-            if (c1 - c0 == strips) {
-                finish<DT>(p, row, a, top.key);
-            } else {
-                // the CTAs whose runs hold this row's first and last strips
-                const int64_t r0 = row * strips, r1 = r0 + strips - 1;
-                const int64_t first = ((r0 + 1) * grid - 1) / total, last = ((r1 + 1) * grid - 1) / total;
-                ScorePart * part = p.parts + 2 * cta + (x == begin ? 0 : 1);
+            a = lane < kWarps ? stats[lane] : stat_empty();
+            a = warp_join(a);
+        }
+        const unsigned long long mine = tid < n_top ? keys.key[tid] : 0ull;
+        if (c1 - c0 == strips) {
+            if (warp == 0) finish<DT>(p, row, a, mine);
+        } else {
+            // the CTAs whose runs hold this row's first and last strips
+            const int64_t r0 = row * strips;
+            const int from = (int) (((r0 + 1) * grid - 1) / total), upto = (int) (((r0 + strips) * grid - 1) / total);
+            if (warp == 0) {
+                ScorePart * part = p.parts + 2 * cta + (at == begin ? 0 : 1);
                 if (lane == 0) {
                     part->m = a.m;
                     part->s = a.s;
                     part->t = a.t;
                 }
-                if (lane < n_top) part->top[lane] = top.key;
+                if (lane < n_top) part->top[lane] = mine;
                 __threadfence();
                 __syncwarp();
-                int seen = 0;
-                if (lane == 0) seen = atomicAdd(&p.counters[first], 1);
-                seen = __shfl_sync(kAll, seen, 0);
-                if (seen == (int) (last - first)) {
-                    __threadfence();
-                    Stat sum = stat_empty();
-                    top.clear(n_top);
-                    for (int64_t b0 = first; b0 <= last; b0 += 32) {
-                        const int64_t b = b0 + lane;
-                        Stat one = stat_empty();
-                        if (b <= last) {
-                            const bool mid = b == first && b * total / grid != r0;
-                            const ScorePart * q = p.parts + 2 * b + (mid ? 1 : 0);
-                            one = {__ldcg(&q->m), __ldcg(&q->s), __ldcg(&q->t)};
-                        }
-                        sum = stat_join(sum, warp_join(one));
+                if (lane == 0) arrived = atomicAdd(&p.counters[from], 1);
+            }
+            __syncthreads();
+            if (arrived == upto - from) {
+                __threadfence();
+                auto part_of = [&](int b) {
+                    const bool mid = b == from && b * total / grid != r0;
+                    return p.parts + 2 * b + (mid ? 1 : 0);
+                };
+                // the n_top-th largest of the parts' largest keys bounds the list from below
+                if (tid == 0) {
+                    keys.bound = 0ull;
+                    keys.warm = 0u;
+                    keys.count = 0;
+                }
+                Stat one = stat_empty();
+                unsigned long long most = 0ull;
+                for (int b0 = from; b0 <= upto; b0 += kThreads) {
+                    const int b = b0 + tid;
+                    if (b <= upto) {
+                        const ScorePart * q = part_of(b);
+                        one = stat_join(one, Stat{__ldcg(&q->m), __ldcg(&q->s), __ldcg(&q->t)});
+                        if (n_top) most = max(most, __ldcg(&q->top[0]));
                     }
-                    for (int64_t b0 = first; n_top && b0 <= last; b0 += 32) {
-                        const int64_t b = b0 + lane;
-                        const bool mid = b == first && b * total / grid != r0;
-                        const ScorePart * q = p.parts + 2 * b + (mid ? 1 : 0);
-                        for (int j = 0; j < n_top; ++j) {  // the parts' lists are in order
-                            const unsigned long long k = b <= last ? __ldcg(&q->top[j]) : 0ull;
-                            if (j == 0 && top.low == 0ull) top.bound((uint32_t) (k >> 32));
-                            if (!__any_sync(kAll, k > top.low)) break;
-                            top.offer(k);
-                        }
+                }
+                one = warp_join(one);
+                if (lane == 0) stats[warp] = one;
+                keys.group[tid] = most;
+                __syncthreads();
+                if (n_top && most) {
+                    int above = 0;
+                    const int parts = min(kThreads, upto - from + 1);
+                    for (int j = 0; j < parts; ++j) above += keys.group[j] > most;
+                    if (above == n_top - 1) keys.bound = most;
+                }
+                __syncthreads();
+                // at most 1024 keys at a time
+                const int step = n_top ? 1024 / kMaxTop : upto - from + 1;
+                for (int b0 = from; n_top && b0 <= upto; b0 += step) {
+                    for (int i = tid; i < step * n_top; i += kThreads) {
+                        const int b = b0 + i / n_top;
+                        if (b > upto) break;
+                        const unsigned long long k = __ldcg(&part_of(b)->top[i % n_top]);
+                        if (k && k >= keys.bound) keys.key[atomicAdd(&keys.count, 1)] = k;
                     }
-                    if (lane == 0) p.counters[first] = 0;
-                    finish<DT>(p, row, sum, top.key);
+                    __syncthreads();
+                    rank_kept(keys, n_top);
+                }
+                if (warp == 0) {
+                    one = warp_join(lane < kWarps ? stats[lane] : stat_empty());
+                    if (lane == 0) p.counters[from] = 0;
+                    finish<DT>(p, row, one, lane < n_top ? keys.key[lane] : 0ull);
                 }
             }
         }
         __syncthreads();
-        x += c1 - c0;
+        at += c1 - c0;
     }
 }
 
 template <int DT>
 cudaError_t launch(ScoreLogitsParams & p, int sms, cudaStream_t stream) {
-    if (p.out.vocab <= kThreads * kPer) {
+    if (p.out.vocab <= kRowOfWarp) {
         score_warp_kernel<DT><<<(unsigned) ((p.rows + kWarps - 1) / kWarps), kThreads, 0, stream>>>(p);
         return cudaGetLastError();
     }
     const int64_t n_vec = p.out.vocab / Elem<DT>::kVec;
     p.strips = (n_vec + kThreads * Elem<DT>::kLoads - 1) / (kThreads * Elem<DT>::kLoads);
-    const int64_t grid = std::min<int64_t>(p.strips * p.rows, (int64_t) sms * kScoreCtasPerSm);
-    score_block_kernel<DT><<<(unsigned) grid, kThreads, 0, stream>>>(p);
+    const int64_t grid = std::min<int64_t>(p.strips * p.rows, (int64_t) sms * ctas_per_sm(p.out.n_top > 0));
+    constexpr int kRing = kStages * kThreads * Elem<DT>::kLoads * 16;
+    auto kernel = p.out.n_top > 0 ? score_block_kernel<DT, true> : score_block_kernel<DT, false>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned) grid, kThreads, kRing, stream>>>(p);
     return cudaGetLastError();
 }
 

@@ -115,6 +115,15 @@ __device__ __forceinline__ float top_value(unsigned long long key) {
     return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
+// The next value below that of `bits` (a key's upper half), NaN where there is none: a
+// comparison with it passes what the bits allow.
+__device__ __forceinline__ float top_below(uint32_t bits) {
+    if (bits <= 1u) return __uint_as_float(0x7fc00000u);
+    --bits;
+    if (bits == 0x7fffffffu) --bits;  // -0 is 0 here
+    return top_value((unsigned long long) bits << 32);
+}
+
 // A list held by a warp, its j-th largest key in lane j.
 struct WarpTop {
     unsigned long long key;  // this lane's

@@ -108,6 +108,14 @@ __device__ __forceinline__ void tc_drain(uint64_t * bar, uint32_t parity) {
     }
 }
 
+// Bulk copy of consecutive bytes (16-byte aligned, a multiple of 16), counted on a barrier.
+__device__ __forceinline__ void bulk_load(void * dst, const void * src, uint32_t bytes, uint64_t * bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 // 2-D TMA tile load into this CTA's shared memory.  In a pair its bytes are counted
 // on the barrier of the pair's first CTA (address bit 24 names the odd one).
 template <int CG>
