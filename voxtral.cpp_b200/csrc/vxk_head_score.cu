@@ -40,8 +40,12 @@ namespace vxk {
 namespace {
 
 constexpr int kThreads = 384;
-// Registers a thread after the split: 128 x 40 + 256 x 232 = 384 x 168, the launch's.
-constexpr int kRegsIssue = 40, kRegsEpilogue = 232;
+// Registers a thread after the split: 128 x 40 + 256 x 232 = 128 x 24 + 256 x 240 = 384 x 168,
+// the launch's; which of the two leaves no role spilling goes by the list.
+template <int LIST>
+constexpr int kRegsIssue = LIST ? 40 : 24;
+template <int LIST>
+constexpr int kRegsEpilogue = LIST ? 232 : 240;
 constexpr int kChunk = 64;                      // columns of x and W in a stage (one 128-byte row)
 constexpr int kXBytes = 128 * 128;              // a CTA's rows of x in a stage
 constexpr int kHalfCols = 128;                  // most columns of a tile in one epilogue thread
@@ -138,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(base + kOffBar + 8 * S::kBars);
     volatile int32_t * abort_flag = reinterpret_cast<volatile int32_t *>(base + kOffBar + 8 * S::kBars + 4);
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = (int) uniform(tid >> 5), lane = tid & 31;
     const int rank = CG == 2 ? (int) cluster_rank() : 0;
     const int unit = (int) blockIdx.x / CG;
     const int row_tile = unit % p.n_row_tiles, group = unit / p.n_row_tiles;
@@ -164,11 +168,11 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
     __syncthreads();
     if constexpr (CG == 2) cluster_sync();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue<LIST>));
         if (warp == 0 && lane == 0) {
             const int w_rows = p.tile_cols / CG;
             const uint32_t bytes = (uint32_t) (p.x_box_rows + w_rows) * 128;
@@ -204,44 +208,46 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                 for (uint32_t d = c > (uint32_t) S::kStages ? c - S::kStages : 0; d < c; ++d)
                     tc_drain(&bars[S::kFull + d % S::kStages], (d / S::kStages) & 1);
         }
-        if (warp == 1 && lane == 0 && rank == 0) {
+        if (warp == 1 && rank == 0) {
             constexpr uint32_t fmt = DT == 30 ? 1u : 0u;
             const uint32_t idesc = tc_idesc(fmt, 128 * CG, p.tile_cols);
-            uint32_t c = 0, seg = 0;
+            const uint32_t ring = smem_u32(base);
+            uint32_t st = 0, par = 0, seg = 0;
             bool ok = true;
             for (int tile = group; ok && tile < p.n_tiles; tile += p.n_groups) {
                 for (int s = 0; ok && s < n_segs; ++s, ++seg) {
-                    const int b = (int) (seg & 1);
-                    if (!tc_wait(&bars[S::kDEmpty + b], ((seg >> 1) & 1) ^ 1, abort_flag, p.error)) {
-                        ok = false;
-                        break;
-                    }
+                    const uint32_t b = seg & 1;
+                    ok = uniform(tc_wait(&bars[S::kDEmpty + b], ((seg >> 1) & 1) ^ 1, abort_flag, p.error));
+                    if (!ok) break;
                     tc_fence_after();
                     const uint32_t d = tmem + 256 * b;
                     const int last = min(n_chunks, (s + 1) * kSegment);
-                    for (int ch = s * kSegment; ch < last; ++ch, ++c) {
-                        const int st = (int) (c % S::kStages);
-                        if (!tc_wait(&bars[S::kFull + st], (c / S::kStages) & 1, abort_flag, p.error)) {
-                            ok = false;
-                            break;
-                        }
+                    for (int ch = s * kSegment; ch < last; ++ch) {
+                        ok = uniform(tc_wait(&bars[S::kFull + st], par, abort_flag, p.error));
+                        if (!ok) break;
                         tc_fence_after();
-                        const uint32_t xa = smem_u32(base + st * S::kStageBytes);
+                        const uint32_t xa = ring + st * S::kStageBytes;
                         const uint64_t da = sw128_desc(xa, 16, 1024), db = sw128_desc(xa + kXBytes, 16, 1024);
+                        if (elect_one()) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)  // 32 bytes further: 2 in the descriptor's 16-byte units
-                            tc_mma<CG>(d, da + 2 * ks, db + 2 * ks, idesc, (ch != s * kSegment) | (ks != 0));
-                        tc_commit<CG>(&bars[S::kEmpty + st]);
+                            for (int ks = 0; ks < 4; ++ks)  // 32 bytes further: 2 in the descriptor's 16-byte units
+                                tc_mma<CG>(d, da + 2 * ks, db + 2 * ks, idesc, (ch != s * kSegment) | (ks != 0));
+                            tc_commit<CG>(&bars[S::kEmpty + st]);
+                            if (ch + 1 == last) tc_commit<CG>(&bars[S::kDFull + b]);
+                        }
+                        __syncwarp();
+                        if (++st == S::kStages) st = 0, par ^= 1;
                     }
-                    if (ok) tc_commit<CG>(&bars[S::kDFull + b]);
                 }
             }
-            tc_commit<CG>(&bars[S::kDrain]);
-            tc_drain(&bars[S::kDrain], 0);
+            if (elect_one()) {
+                tc_commit<CG>(&bars[S::kDrain]);
+                tc_drain(&bars[S::kDrain], 0);
+            }
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue<LIST>));
         const int q = warp & 3, half = (warp - 4) >> 2;
         const int t = half * 128 + q * 32 + lane;   // this thread's place in the lists
         const int row = row0 + q * 32 + lane;
@@ -259,11 +265,10 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
         asm volatile("griddepcontrol.wait;" ::: "memory");
         const int32_t token = p.tokens && row < p.n_rows ? p.tokens[row] : -1;
         Stat a = stat_empty();
-        uint32_t seg = 0;
+        uint32_t seg = 0;  // two accumulators in turn: bit 0, and the parity in bit 1
         bool have = true;
         for (int tile = group; have && tile < p.n_tiles; tile += p.n_groups) {
             float acc[kHalfCols];
-            uint32_t bound = listed && tile != group ? __ldcg(&p.row_low[row]) : 0u;
             for (int s = 0; s < n_segs; ++s, ++seg) {
                 const int b = (int) (seg & 1);
                 have = __all_sync(kAll, tc_wait(&bars[S::kDFull + b], (seg >> 1) & 1, abort_flag, p.error));
@@ -281,6 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                 if (lane == 0) mbar_arrive_cluster<CG>(&bars[S::kDEmpty + b], 0);
             }
             if (!have) break;
+            // the row's bound so far, on its way while the statistics are taken
+            uint32_t bound = listed && tile != group ? __ldcg(&p.row_low[row]) : 0u;
             const int col0 = tile * p.tile_cols + half * n_half;
             const int limit = min(n_half, p.vocab - col0);
             if (limit < kHalfCols) {
@@ -340,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                     low = top_below(bound);
                 }
                 if (!(m <= low)) {
-                    const unsigned long long before = low_key;
+                    bool raised = false;
 #pragma unroll
                     for (int g = 0; g < 16; ++g) {
                         if (!(most[g] <= low)) {
@@ -362,12 +369,13 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                                     if (end > low_key) {
                                         low_key = end;
                                         low = top_value(end);
+                                        raised = true;
                                     }
                                 }
                             }
                         }
                     }
-                    if (low_key > before) atomicMax(&p.row_low[row], (uint32_t) (low_key >> 32));
+                    if (raised) atomicMax(&p.row_low[row], (uint32_t) (low_key >> 32));
                 }
             }
         }

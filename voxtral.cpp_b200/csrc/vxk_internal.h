@@ -348,6 +348,7 @@ struct PromptAttnParams {
     int32_t causal, window;
     int32_t pack_shift;          // log2 of the heads in one tile
     int32_t tokens;              // tokens in one tile: 128 >> pack_shift
+    int32_t out_32;              // out is 32-byte aligned
     float scale_log2;            // softmax scale * log2(e)
     const void * v;
     void * out;

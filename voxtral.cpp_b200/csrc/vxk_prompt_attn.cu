@@ -35,8 +35,8 @@ namespace vxk {
 namespace {
 
 constexpr int kThreads = 384;
-// Registers a thread after the split: 128 x 56 + 256 x 224 = 384 x 168, the launch's.
-constexpr int kRegsIssue = 56, kRegsSoftmax = 224;
+// Registers a thread after the split: 128 x 72 + 256 x 216 = 384 x 168, the launch's.
+constexpr int kRegsIssue = 72, kRegsSoftmax = 216;
 constexpr int kTile = 128;        // query rows and keys of a tile
 constexpr int kFlags = 16;        // items that the V warps may be ahead of the epilogue
 constexpr float kSlack = 8.0f;    // growth of c m that is let pass without a rescale
@@ -49,7 +49,8 @@ struct Shape {
     static constexpr int kOffBar = kOffRing + kStages * kTileBytes;
     // barriers
     static constexpr int kFull = 0, kEmpty = kStages, kReady = 2 * kStages, kQFull = 3 * kStages, kQEmpty = kQFull + 2,
-                         kSFull = kQEmpty + 2, kPFull = kSFull + 2, kODone = kPFull + 2, kDrain = kODone + 2;
+                         kSFull = kQEmpty + 2, kPFull = kSFull + 2, kODone = kPFull + 4, kOHalf = kODone + 2,
+                         kDrain = kOHalf + 2;
     static constexpr int kBars = kDrain + 1;
     static constexpr int kOffMisc = kOffBar + 8 * kBars;  // TMEM base, abort flag, V flags
     static constexpr int kSmem = kOffMisc + 8 + 2 * kFlags * 4 + 1024;
@@ -128,6 +129,13 @@ __device__ __forceinline__ bool not_finite(uint16_t v) {
     return (v & e) == e;
 }
 
+// Of two such values: all ones in each finite one's half.
+template <int DT>
+__device__ __forceinline__ uint32_t finite_mask(uint32_t w) {
+    constexpr uint32_t e = DT == 30 ? 0x7f807f80u : 0x7c007c00u;
+    return __vcmpne2(w & e, e);
+}
+
 // Shared-memory descriptors (vxk_tc.h) in halves: the upper one is the same for every
 // operand here (1024 bytes from one group of eight rows to the next, 128-byte swizzle), the
 // lower one holds the address and, for V, the 16 KB from one 64 dims to the next.
@@ -192,8 +200,109 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t * r)
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
         : "memory");
 }
+// 32 bytes to a 32-byte aligned address.
+__device__ __forceinline__ void store_32(void * to, const uint32_t * v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// p = 2^(c x + off) of 32 scores, added to the sums and stored as 16 bits in TMEM.
+template <int DT>
+__device__ __forceinline__ void exp_chunk(const float * x, uint32_t tp, uint64_t c2, uint64_t off2, uint64_t (&total)[2]) {
+    uint32_t h[16];
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+        float a, b;
+        unpair(fma2(pair(x[e], x[e + 1]), c2, off2), a, b);
+        a = ex2f(a);
+        b = ex2f(b);
+        total[e / 2 % 2] = add2(total[e / 2 % 2], pair(a, b));
+        h[e / 2] = cvt2<DT>(a, b);
+    }
+    tmem_store16(tp, h);
+}
+
+// O times f, a row's columns of TMEM at `to`.
+template <int HD>
+__device__ __forceinline__ void scale_o(uint32_t to, float f) {
+#pragma unroll
+    for (int k = 0; k < HD; k += 16) {
+        uint32_t o[16];
+        tmem_load16(to + k, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+        tmem_store16(to + k, o);
+    }
+}
+
+// One thread's running state over the keys of its row.
+struct RowState {
+    float m;             // what p is taken from, in score units
+    float sum;
+};
+
+// 64 scores of a row: the running maximum, p into TMEM at tp, the sum.  hi, lo: the
+// columns [lo, hi) of these that the row attends (MASKED).  Where some row's maximum has
+// outgrown kSlack, grown() is called before anything depends on the new one: it waits for the
+// products so far and multiplies O by its argument.
+template <int DT, bool MASKED, typename F>
+__device__ __forceinline__ bool half_step(float (&x)[64], uint32_t tp, float c, int hi, int lo, RowState & r, F && grown) {
+    bool whole[2] = {true, true}, none[2] = {false, false};
+    if constexpr (MASKED) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            whole[k] = __all_sync(0xffffffffu, hi >= 32 * k + 32 && lo <= 32 * k);
+            none[k] = __all_sync(0xffffffffu, hi <= 32 * k || lo >= 32 * k + 32);
+            if (!whole[k] && !none[k]) {
+#pragma unroll
+                for (int e = 32 * k; e < 32 * k + 32; ++e)
+                    if (e >= hi || e < lo) x[e] = -INFINITY;
+            }
+        }
+    }
+    float mt[4] = {r.m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        if (MASKED && none[k]) continue;
+#pragma unroll
+        for (int e = 32 * k; e < 32 * k + 32; e += 2) mt[e / 2 % 4] = max3(mt[e / 2 % 4], x[e], x[e + 1]);
+    }
+    const float mn = fmaxf(max3(mt[0], mt[1], mt[2]), mt[3]);
+    const bool grow = r.m != -INFINITY && (mn - r.m) * c > kSlack;
+    if (__any_sync(0xffffffffu, grow)) {
+        const float f = grow ? ex2f((r.m - mn) * c) : 1.0f;
+        r.sum *= f;
+        if (grow) r.m = mn;
+        if (!grown(f)) return false;
+    }
+    if (r.m == -INFINITY) r.m = mn;                  // nothing in O or the sum yet
+    const float off = r.m == -INFINITY ? 0.0f : -r.m * c;
+    const uint64_t c2 = pair(c, c), off2 = pair(off, off);
+    uint64_t total[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        if (MASKED && none[k]) {
+            const uint32_t zero[16] = {};
+            tmem_store16(tp + 16 * k, zero);
+        } else {
+            exp_chunk<DT>(x + 32 * k, tp + 16 * k, c2, off2, total);
+        }
+    }
+    float a, b;
+    unpair(add2(total[0], total[1]), a, b);
+    r.sum += a + b;
+    return true;
+}
 
 template <int DT, int HD>
 __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __grid_constant__ CUtensorMap tmq,
@@ -209,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
     volatile int32_t * abort_flag = reinterpret_cast<volatile int32_t *>(base + S::kOffMisc + 4);
     volatile int32_t * v_flags = reinterpret_cast<volatile int32_t *>(base + S::kOffMisc + 8);  // [2 warps][kFlags]
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = (int) uniform(tid >> 5), lane = tid & 31;
     const int4 head = *reinterpret_cast<const int4 *>(p.plan);
     if (head.y > p.rows) {  // a replay under a plan larger than the buffers
         if (tid == 0 && blockIdx.x == 0) atomicCAS(p.error, 0, kErrPlan);
@@ -230,8 +339,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             mbar_init(&bars[S::kQFull + s], 1);
             mbar_init(&bars[S::kQEmpty + s], 1);
             mbar_init(&bars[S::kSFull + s], 1);
-            mbar_init(&bars[S::kPFull + s], 4);
+            mbar_init(&bars[S::kPFull + 2 * s], 4);  // keys 0-63
+            mbar_init(&bars[S::kPFull + 2 * s + 1], 4);
             mbar_init(&bars[S::kODone + s], 1);
+            mbar_init(&bars[S::kOHalf + s], 1);
         }
         mbar_init(&bars[S::kDrain], 1);
         *abort_flag = 0;
@@ -241,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
@@ -284,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                 tc_drain(&bars[S::kFull + d % S::kStages], (d / S::kStages) & 1);
             for (int s = 0; s < 2; ++s)
                 if (cq[s]) tc_drain(&bars[S::kQFull + s], (cq[s] - 1) & 1);
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
             // ---------------- tcgen05.mma issuer ----------------
             constexpr uint32_t fmt = DT == 30 ? 1u : 0u;
             constexpr uint32_t idesc_s = tc_idesc(fmt, kTile, kTile), idesc_o = tc_idesc(fmt, kTile, HD, 1);
@@ -297,74 +408,99 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                 const bool have = tc_wait(&bars[bar], (bits & bit) != 0, abort_flag, p.error);
                 tc_fence_after();
                 bits ^= bit;
-                return have;
+                return (bool) uniform(have);
             };
             auto wait_tile = [&](uint32_t at, uint32_t parity) {
                 const bool have = tc_wait(&bars[S::kReady + at], parity, abort_flag, p.error);
                 tc_fence_after();
-                return have;
+                return (bool) uniform(have);
             };
-            auto scores = [&](int s, uint32_t at) {
-                const uint32_t dq = desc_lo(smem_u32(base) + s * S::kTileBytes, 16);
-                const uint32_t dk = desc_lo(smem_u32(ring) + at * S::kTileBytes, 16);
+            const uint32_t sm_q = desc_lo(smem_u32(base), 16), sm_k = desc_lo(smem_u32(ring), 16),
+                           sm_v = desc_lo(smem_u32(ring), kTile * 128);
+            constexpr uint32_t kTileDesc = S::kTileBytes >> 4;
+            // S of a tile from the keys in place `at`; then what the scores were the last to use
+            auto scores = [&](int s, uint32_t at, bool last) {
+                const uint32_t dq = sm_q + s * kTileDesc, dk = sm_k + at * kTileDesc;
+                if (elect_one()) {
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {  // 64 dims are 16 KB of the tile
-                    const uint32_t step = (uint32_t) ((ks / 4) * (kTile * 128) + (ks % 4) * 32) >> 4;
-                    mma_ss(tmem + s * kTile, dq + step, dk + step, idesc_s, ks != 0);
+                    for (int ks = 0; ks < HD / 16; ++ks) {  // 64 dims are 16 KB of the tile
+                        const uint32_t step = (uint32_t) ((ks / 4) * (kTile * 128) + (ks % 4) * 32) >> 4;
+                        mma_ss(tmem + s * kTile, dq + step, dk + step, idesc_s, ks != 0);
+                    }
+                    tc_commit<1>(&bars[S::kSFull + s]);
+                    if (last) tc_commit<1>(&bars[S::kQEmpty + s]);
                 }
-                tc_commit<1>(&bars[S::kSFull + s]);
+                __syncwarp();
+            };
+            auto release = [&](uint32_t at) {
+                if (elect_one()) tc_commit<1>(&bars[S::kEmpty + at]);
+                __syncwarp();
             };
             for (int i = begin; ok && i < end; ++i) {
                 Item it;
                 it.set(items[i], p);
-                const int n = it.tiles();
+                const int n0 = (int) uniform(it.n[0]), n1 = (int) uniform(it.n[1]), n = max(n0, n1);
                 ok = wait_tile(st, par);
-#pragma unroll 1
-                for (int s = 0; ok && s < 2; ++s) {
-                    const int ns = s ? it.n[1] : it.n[0];
-                    if (ns == 0) continue;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const int ns = s ? n1 : n0;
+                    if (!ok || ns == 0) continue;
                     ok = wait_bit(S::kQFull + s, kBitQ << s);
-                    if (!ok) break;
-                    scores(s, st);
-                    if (ns == 1) tc_commit<1>(&bars[S::kQEmpty + s]);
+                    if (ok) scores(s, st, ns == 1);
                 }
-                if (ok) tc_commit<1>(&bars[S::kEmpty + st]);
+                if (!ok) break;
+                release(st);
                 for (int j = 0; ok && j < n; ++j) {
                     if (++st == S::kStages) st = 0, par ^= 1;       // V of these keys
                     uint32_t st_k = st + 1, par_k = par;            // K of the next
                     if (st_k == S::kStages) st_k = 0, par_k ^= 1;
+                    const uint32_t dv = sm_v + st * kTileDesc;
                     bool have_v = false, have_k = false;
-#pragma unroll 1
-                    for (int s = 0; ok && s < 2; ++s) {
-                        const int ns = s ? it.n[1] : it.n[0];
-                        if (j < ns) {
-                            ok = wait_bit(S::kPFull + s, kBitP << s);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const int ns = s ? n1 : n0;
+                        if (ok && j < ns) {
+                            const uint32_t d = tmem + 2 * kTile + s * HD, a = tmem + s * kTile;
+                            ok = wait_bit(S::kPFull + 2 * s, kBitP << s);
                             if (ok && !have_v) ok = wait_tile(st, par);
                             have_v = true;
                             if (!ok) break;
-                            const uint32_t dv = desc_lo(smem_u32(ring) + st * S::kTileBytes, kTile * 128);
+                            if (elect_one()) {
 #pragma unroll
-                            for (int ks = 0; ks < kTile / 16; ++ks)  // 16 keys: 8 columns of P, 2 KB of V
-                                mma_ts(tmem + 2 * kTile + s * HD, tmem + s * kTile + 8 * ks, dv + 128 * ks, idesc_o,
-                                       (j | ks) != 0);
-                            tc_commit<1>(&bars[S::kODone + s]);
+                                for (int ks = 0; ks < kTile / 32; ++ks)  // 16 keys: 8 columns of P, 2 KB of V
+                                    mma_ts(d, a + 8 * ks, dv + 128 * ks, idesc_o, (j | ks) != 0);
+                                tc_commit<1>(&bars[S::kOHalf + s]);
+                            }
+                            __syncwarp();
+                            bits ^= kBitP << s;  // the second half's barrier has the first's parity
+                            ok = wait_bit(S::kPFull + 2 * s + 1, kBitP << s);
+                            if (!ok) break;
+                            if (elect_one()) {
+#pragma unroll
+                                for (int ks = kTile / 32; ks < kTile / 16; ++ks)
+                                    mma_ts(d, a + 8 * ks, dv + 128 * ks, idesc_o, 1);
+                                tc_commit<1>(&bars[S::kODone + s]);
+                            }
+                            __syncwarp();
                         }
-                        if (j + 1 < ns) {
+                        if (ok && j + 1 < ns) {
                             if (!have_k) ok = wait_tile(st_k, par_k);
                             have_k = true;
                             if (!ok) break;
-                            scores(s, st_k);
-                            if (j + 2 == ns) tc_commit<1>(&bars[S::kQEmpty + s]);
+                            scores(s, st_k, j + 2 == ns);
                         }
                     }
                     if (!ok) break;
-                    tc_commit<1>(&bars[S::kEmpty + st]);
-                    if (j + 1 < n) tc_commit<1>(&bars[S::kEmpty + st_k]);
+                    release(st);
+                    if (j + 1 < n) release(st_k);
                     st = st_k, par = par_k;
                 }
             }
-            tc_commit<1>(&bars[S::kDrain]);
-            tc_drain(&bars[S::kDrain], 0);
+            if (elect_one()) {
+                tc_commit<1>(&bars[S::kDrain]);
+                tc_drain(&bars[S::kDrain], 0);
+            }
+            __syncwarp();
         } else if (warp >= 2) {
             // ---------------- V rows under a mask ----------------
             // These warps see every tile in turn, masked or not, and pass it on to the issuer:
@@ -385,19 +521,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                         uint4 * v = reinterpret_cast<uint4 *>(ring + st * S::kTileBytes);
                         const int rows = it.len - (it.lo + (j >> 1)) * kTile;
                         for (int q = t; q < S::kTileBytes / 16; q += 64) {
-                            uint4 x = v[q];
-                            const bool behind = q / 8 % kTile >= rows;
-                            uint16_t * h = reinterpret_cast<uint16_t *>(&x);
-                            bool change = behind;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                if (not_finite<DT>(h[e])) {
-                                    change = true;
-                                    bad |= !behind;
-                                    h[e] = 0;
-                                }
+                            if (q / 8 % kTile >= rows) {
+                                v[q] = make_uint4(0, 0, 0, 0);
+                                continue;
                             }
-                            if (change) v[q] = behind ? make_uint4(0, 0, 0, 0) : x;
+                            uint4 x = v[q];
+                            const uint4 f = make_uint4(finite_mask<DT>(x.x), finite_mask<DT>(x.y), finite_mask<DT>(x.z),
+                                                       finite_mask<DT>(x.w));
+                            if ((f.x & f.y & f.z & f.w) != 0xffffffffu) {
+                                bad = true;
+                                v[q] = make_uint4(x.x & f.x, x.y & f.y, x.z & f.z, x.w & f.w);
+                            }
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         bad = __any_sync(0xffffffffu, bad);
@@ -427,75 +561,44 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             const int first = it.t0 + s * p.tokens;
             const int token = first + (r >> p.pack_shift);
             const int last = min(first + p.tokens, it.len) - 1;
-            float m = -INFINITY;                             // what p is taken from, in score units
-            float sum = 0.0f;
+            RowState row = {-INFINITY, 0.0f};
             for (int j = 0; j < n; ++j, ++cs) {
                 ok = __all_sync(0xffffffffu, tc_wait(&bars[S::kSFull + s], cs & 1, abort_flag, p.error));
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t raw[kTile];
-#pragma unroll
-                for (int k = 0; k < kTile; k += 32) tmem_load32(ts + k, raw + k);
-                tmem_wait_ld();
-                float x[kTile];
-#pragma unroll
-                for (int k = 0; k < kTile; ++k) x[k] = __uint_as_float(raw[k]);
+                float x[64];
+                tmem_load32(ts, reinterpret_cast<uint32_t *>(x));
+                tmem_load32(ts + 32, reinterpret_cast<uint32_t *>(x) + 32);
                 const int k0 = (it.lo + j) * kTile;
-                if (k0 + kTile > (p.causal ? min(first + 1, it.len) : it.len) || (p.window > 0 && last - p.window >= k0)) {
-                    const int hi = (p.causal ? min(token + 1, it.len) : it.len) - k0;
-                    const int lo = p.window > 0 ? token - p.window + 1 - k0 : 0;
+                const bool masked =
+                    k0 + kTile > (p.causal ? min(first + 1, it.len) : it.len) || (p.window > 0 && last - p.window >= k0);
+                const int hi = (p.causal ? min(token + 1, it.len) : it.len) - k0;
+                const int lo = p.window > 0 ? token - p.window + 1 - k0 : 0;
 #pragma unroll
-                    for (int k = 0; k < kTile; ++k)
-                        if (k >= hi || k < lo) x[k] = -INFINITY;
-                }
-                float mt[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int k = 4; k < kTile; ++k) mt[k % 4] = fmaxf(mt[k % 4], x[k]);
-                const float mn = fmaxf(m, fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3])));
-                const bool grow = m != -INFINITY && (mn - m) * c > kSlack;
-                if (__any_sync(0xffffffffu, grow)) {
-                    // O of this tile: its last product has to be done
-                    ok = __all_sync(0xffffffffu, tc_wait(&bars[S::kODone + s], (cs - 1) & 1, abort_flag, p.error));
+                for (int half = 0; half < 2; ++half) {
+                    tmem_wait_ld();
+                    // O is complete up to the last tile when S is there, and up to this tile's
+                    // first half when that is said to be
+                    auto grown = [&](float f) {
+                        if (half && !__all_sync(0xffffffffu, tc_wait(&bars[S::kOHalf + s], cs & 1, abort_flag, p.error)))
+                            return false;
+                        tc_fence_after();
+                        if (j + half > 0) scale_o<HD>(to, f);
+                        return true;
+                    };
+                    ok = masked ? half_step<DT, true>(x, ts + 32 * half, c, hi - 64 * half, lo - 64 * half, row, grown)
+                                : half_step<DT, false>(x, ts + 32 * half, c, 0, 0, row, grown);
                     if (!ok) break;
-                    tc_fence_after();
-                    const float f = grow ? ex2f((m - mn) * c) : 1.0f;
-                    sum *= f;
-#pragma unroll
-                    for (int k = 0; k < HD; k += 16) {
-                        uint32_t o[16];
-                        tmem_load16(to + k, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_store16(to + k, o);
+                    tmem_wait_st();
+                    if (half == 0) {  // under way while the first half is handed over
+                        tmem_load32(ts + 64, reinterpret_cast<uint32_t *>(x));
+                        tmem_load32(ts + 96, reinterpret_cast<uint32_t *>(x) + 32);
                     }
-                    if (grow) m = mn;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars[S::kPFull + 2 * s + half]);
                 }
-                if (m == -INFINITY) m = mn;                  // nothing in O or the sum yet
-                const float off = m == -INFINITY ? 0.0f : -m * c;
-                const uint64_t c2 = pair(c, c), off2 = pair(off, off);
-                uint64_t total[2] = {0, 0};
-#pragma unroll
-                for (int k = 0; k < kTile; k += 32) {
-                    uint32_t h[16];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float a, b;
-                        unpair(fma2(pair(x[k + e], x[k + e + 1]), c2, off2), a, b);
-                        a = ex2f(a);
-                        b = ex2f(b);
-                        total[e / 2 % 2] = add2(total[e / 2 % 2], pair(a, b));
-                        h[e / 2] = cvt2<DT>(a, b);
-                    }
-                    tmem_store16(ts + k / 2, h);
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars[S::kPFull + s]);
-                float a, b;
-                unpair(add2(total[0], total[1]), a, b);
-                sum += a + b;
+                if (!ok) break;
             }
             if (!ok) break;
             // epilogue: O / sum
@@ -504,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             tc_fence_after();
             const bool bad = v_flags[(i - begin) % kFlags] | v_flags[kFlags + (i - begin) % kFlags];
             const int head = it.head + (r & ((1 << p.pack_shift) - 1));
-            const float f = 1.0f / sum;
+            const float f = 1.0f / row.sum;
             uint16_t * out = static_cast<uint16_t *>(p.out) + ((int64_t) (it.row0 + token) * p.n_q + head) * HD;
 #pragma unroll
             for (int k = 0; k < HD; k += 32) {
@@ -532,11 +635,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                             }
                         }
                     }
+                    uint32_t h[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4 *>(out + k + e) =
-                            make_uint4(cvt2<DT>(y[e], y[e + 1]), cvt2<DT>(y[e + 2], y[e + 3]), cvt2<DT>(y[e + 4], y[e + 5]),
-                                       cvt2<DT>(y[e + 6], y[e + 7]));
+                    for (int e = 0; e < 16; ++e) h[e] = cvt2<DT>(y[2 * e], y[2 * e + 1]);
+                    if (p.out_32) {  // whole sectors: half the requests
+                        store_32(out + k, h);
+                        store_32(out + k + 16, h + 8);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            *reinterpret_cast<uint4 *>(out + k + 2 * e) = make_uint4(h[e], h[e + 1], h[e + 2], h[e + 3]);
+                    }
                 }
             }
             tc_fence_before();

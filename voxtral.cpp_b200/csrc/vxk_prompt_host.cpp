@@ -378,6 +378,7 @@ vxk_status vxk_prompt_attention(vxk_prompt * prompt, const void * q, const void 
         a.group = c.n_q_heads / c.n_kv_heads;
         a.pack_shift = prompt->pack_shift;
         a.tokens = prompt->tokens;
+        a.out_32 = reinterpret_cast<uintptr_t>(out) % 32 == 0;
         a.head_dim = c.head_dim;
         a.dtype = (int32_t) c.dtype;
         a.causal = c.causal;

@@ -29,6 +29,23 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     return r;
 }
 
+// True in one lane of the warp.  An issuer warp runs as a whole, its values uniform, and
+// only the instructions themselves are one lane's: in a branch that a single lane takes
+// every operand of an MMA is moved to a uniform register first, which takes longer than a
+// 128 x 128 x 16 MMA.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
+// A value that is the same in all lanes, as the compiler can see.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
