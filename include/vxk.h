@@ -809,6 +809,23 @@ VXK_API vxk_status vxk_decoder_get_info(const vxk_decoder * d, vxk_decoder_info 
 VXK_API vxk_status vxk_decoder_forward(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slots,
                                        int32_t * argmax, float * logits, float * hidden, void * cuda_stream);
 
+/**
+ * vxk_decoder_forward that scores every row of the planned batch instead of
+ * predicting behind each stream's last: row r's distribution over the next
+ * token gives the log probability of given[r], its entropy and its n_top most
+ * likely tokens (vxk_head_score; the outputs are its, per row).  With a
+ * transcript's tokens and given[r] = tokens[r + 1] these are the transcript's
+ * word confidences.  Streams that begin with the batch are attended as packed
+ * prompts (vxk_prompt_attention, 16-bit rows), others over the cache
+ * (vxk_attend_layer); either way the caches are appended as in
+ * vxk_decoder_forward and the caller commits, or aborts to leave no trace.
+ *   given  [rows] host array, < vocab; a negative one is not scored
+ * Asynchronous on cuda_stream; the first call allocates its scratch.
+ */
+VXK_API vxk_status vxk_decoder_score(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slots,
+                                     const int32_t * given, int32_t n_top, float * logprob, float * entropy,
+                                     int32_t * top_ids, float * top_logprobs, void * cuda_stream);
+
 /** Writes n encoder-output rows ([n][enc_dim] fp32, device memory) of stream
  *  into its ring at absolute frames frame .. frame+n-1 (slot = frame %
  *  enc_capacity); copy_chunk_to_enc_out_ring (src/voxtral.cpp:4018-4045). */

@@ -100,3 +100,23 @@ def test_score_call_refusals(vxk):
     refused(head.score, a + 8, a, 1, a, 0, a, a, a, a)
     refused(head.score, a, a, 1, a, 17, a, a, a, a)
     head.close()
+
+
+def test_prompt_config_layout_matches_the_c_compiler(vxk, tmp_path):
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    cc = shutil.which("gcc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    names = [f[0] for f in vxk.PromptConfig._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text("#include <stddef.h>\n#include <stdio.h>\n#include <vxk.h>\nint main(void) {\n"
+                   + '    printf("%zu\\n", sizeof(vxk_prompt_config));\n'
+                   + "".join(f'    printf("%zu\\n", offsetof(vxk_prompt_config, {n}));\n' for n in names) + "    return 0;\n}\n")
+    exe = tmp_path / "layout"
+    include = Path(__file__).resolve().parent.parent / "include"
+    subprocess.run([cc, "-std=c11", "-Wall", "-Werror", "-I", str(include), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [C.sizeof(vxk.PromptConfig)] + [getattr(vxk.PromptConfig, n).offset for n in names]

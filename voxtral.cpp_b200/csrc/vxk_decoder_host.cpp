@@ -135,6 +135,12 @@ struct vxk_decoder {
     std::vector<vxk::DecRow> h_rows;
     std::vector<vxk::AdaptRow> h_adapt;
     vxk::PoolBatchView view;
+    // scoring, created by the first vxk_decoder_score
+    vxk_prompt * prompt = nullptr;
+    uint16_t * p16 = nullptr;      // q, k, v and output rows of the packed attention
+    int32_t * d_given = nullptr;   // [max_rows]
+    float * score_logits = nullptr;  // [score_chunk][vocab], quantized heads only
+    int32_t score_chunk = 0;
     std::string last_error;
 };
 
@@ -174,6 +180,9 @@ void destroy(vxk_decoder * d) {
         vxk_qweight_destroy(w);
     }
     if (d->head) vxk_head_destroy(d->head);
+    if (d->prompt) vxk_prompt_destroy(d->prompt);
+    for (void * p : {(void *) d->p16, (void *) d->d_given, (void *) d->score_logits})
+        if (p) cudaFree(p);
     for (void * p : {(void *) d->emb, (void *) d->head_w16_own, (void *) d->attn_norm, (void *) d->ffn_norm,
                      (void *) d->dec_norm, (void *) d->ada, (void *) d->audio, (void *) d->enc, (void *) d->x,
                      (void *) d->xn, (void *) d->q, (void *) d->k, (void *) d->v, (void *) d->att, (void *) d->proj,
@@ -564,10 +573,64 @@ bool norm_into(vxk_decoder * d, vxk::NormParams np, vxk_qweight * const * ws, in
     return false;
 }
 
+// What vxk_decoder_score asks of a forward: every row scored instead of each
+// stream's last one.
+struct ScoreCall {
+    const int32_t * given;  // host, [rows]
+    int32_t n_top;
+    float * logprob;
+    float * entropy;
+    int32_t * top_ids;
+    float * top_logprobs;
+};
+
+// The scoring state of a decoder, allocated once.
+void need_score(vxk_decoder * d) {
+    if (d->prompt) return;
+    const size_t R = (size_t) d->ps.max_rows;
+    const size_t qdim = (size_t) d->ps.n_q * d->ps.head_dim, kvdim = (size_t) d->ps.n_kv * d->ps.head_dim;
+    if (!d->p16) d->p16 = dalloc<uint16_t>(d, R * 2 * (qdim + kvdim));
+    if (!d->d_given) d->d_given = dalloc<int32_t>(d, R);
+    if (d->head_q && !d->score_logits) {
+        // the embeddings are read once per chunk
+        d->score_chunk = std::min<int32_t>(d->chunk, 128);
+        d->score_logits = dalloc<float>(d, (size_t) d->score_chunk * d->vocab);
+    }
+    vxk_prompt_config c = vxk_prompt_default_config();
+    c.device = d->ps.device;
+    c.n_q_heads = d->ps.n_q;
+    c.n_kv_heads = d->ps.n_kv;
+    c.head_dim = d->ps.head_dim;
+    c.max_seqs = d->ps.max_streams;
+    c.max_rows = d->ps.max_rows;
+    c.max_position = 0;  // the rows rotate by the pool's table
+    VXK_DCALL(vxk_prompt_create(&c, &d->prompt), "vxk_prompt_create");
+}
+
+// Log probabilities of `rows` final-normed rows in d->xn.
+void score_rows(vxk_decoder * d, const ScoreCall & sc, int32_t rows, cudaStream_t cs) {
+    const int32_t dim = d->dim;
+    if (!d->head_q) {
+        VXK_DCALL(vxk_head_score(d->head, d->head_w16, d->xn, rows, d->d_given, sc.n_top, sc.logprob, sc.entropy, sc.top_ids,
+                                 sc.top_logprobs, cs),
+                  "vxk_head_score");
+        return;
+    }
+    for (int32_t r0 = 0; r0 < rows; r0 += d->score_chunk) {
+        const int32_t nr = std::min(d->score_chunk, rows - r0);
+        VXK_DCALL(vxk_qweight_matmul(d->head_q, d->xn + (int64_t) r0 * dim, nr, d->score_logits, cs), "quantized logits");
+        VXK_DCALL(vxk_head_score_logits(d->head, d->score_logits, VXK_DTYPE_F32, d->vocab, nr, d->d_given + r0, sc.n_top,
+                                        sc.logprob ? sc.logprob + r0 : nullptr, sc.entropy ? sc.entropy + r0 : nullptr,
+                                        sc.top_ids ? sc.top_ids + (int64_t) r0 * sc.n_top : nullptr,
+                                        sc.top_logprobs ? sc.top_logprobs + (int64_t) r0 * sc.n_top : nullptr, cs),
+                  "vxk_head_score_logits");
+    }
+}
+
 void forward(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slots, int32_t * argmax, float * logits,
-             float * hidden, cudaStream_t cs) {
+             float * hidden, cudaStream_t cs, const ScoreCall * sc = nullptr) {
     if (!vxk::pool_batch_view(d->pool, &d->view)) dfail(VXK_STATUS_INVALID_STATE, "no batch is planned on the pool");
-    if (!tokens || !audio_slots || !argmax) dfail(VXK_STATUS_INVALID_ARGUMENT, "null argument");
+    if (!tokens || !audio_slots || (!argmax && !sc)) dfail(VXK_STATUS_INVALID_ARGUMENT, "null argument");
     const vxk::PoolBatchView & bv = d->view;
     const int32_t rows = (int32_t) bv.row_stream.size();
     const int32_t n_out = (int32_t) bv.last_rows.size();
@@ -580,6 +643,21 @@ void forward(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slot
     }
     for (int32_t i = 0; i < n_out; ++i) d->h_rows[(size_t) bv.last_rows[(size_t) i]].out_index = i;
     DevScope scope(d->ps.device);
+    bool packed = false;  // scoring whole prompts: attention within the batch, not over the cache
+    if (sc) {
+        for (int32_t r = 0; r < rows; ++r)
+            if (sc->given[r] >= d->vocab) dfail(VXK_STATUS_INVALID_ARGUMENT, "given token out of range");
+        need_score(d);
+        upload(d, sc->given, (size_t) rows * sizeof(int32_t), d->d_given, cs);
+        // Streams that begin with this batch attend its rows alone.
+        packed = !bv.single_token;
+        std::vector<int32_t> lens;
+        for (int32_t i = 0, r0 = 0; i < n_out; r0 = bv.last_rows[(size_t) i] + 1, ++i) {
+            lens.push_back(bv.last_rows[(size_t) i] + 1 - r0);
+            packed = packed && bv.row_pos[(size_t) r0] == 0;
+        }
+        if (packed) VXK_DCALL(vxk_prompt_plan(d->prompt, lens.data(), nullptr, n_out, cs), "vxk_prompt_plan");
+    }
     upload(d, d->h_rows.data(), (size_t) rows * sizeof(vxk::DecRow), d->d_rows, cs);
 
     const int32_t dim = d->dim, qdim = d->ps.n_q * d->ps.head_dim, kvdim = d->ps.n_kv * d->ps.head_dim;
@@ -624,7 +702,18 @@ void forward(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slot
             VXK_DCALL(vxk_decode_layer(d->pool, l, d->q, d->k, d->v, d->att, cs), "vxk_decode_layer");
         } else {
             VXK_DCALL(vxk_append_layer(d->pool, l, d->k, d->v, cs), "vxk_append_layer");
-            VXK_DCALL(vxk_attend_layer(d->pool, l, d->q, d->att, cs), "vxk_attend_layer");
+            if (packed) {
+                const size_t R = (size_t) rows;
+                uint16_t *q16 = d->p16, *o16 = q16 + R * qdim, *k16 = o16 + R * qdim, *v16 = k16 + R * kvdim;
+                int32_t table_rows = 0;
+                const float2 * table = vxk::pool_rope_table(d->pool, &table_rows);
+                VXK_DCALL((vxk_status) vxk::prompt_rope_with(d->prompt, table, table_rows, d->q, d->k, d->v, q16, k16, v16, cs),
+                          "vxk_prompt_rope");
+                VXK_DCALL(vxk_prompt_attention(d->prompt, q16, k16, v16, o16, cs), "vxk_prompt_attention");
+                VXK_DCUDA(vxk::launch_widen(o16, d->att, (int64_t) rows * qdim, VXK_DTYPE_F16, cs));
+            } else {
+                VXK_DCALL(vxk_attend_layer(d->pool, l, d->q, d->att, cs), "vxk_attend_layer");
+            }
         }
         {
             float * ys[1] = {d->proj};
@@ -665,8 +754,8 @@ void forward(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slot
         const bool last = l + 1 == d->n_layers;
         np.w = last ? d->dec_norm : d->attn_norm + (int64_t) (l + 1) * dim;
         np.ada = nullptr;
-        np.out = last ? d->hn : d->xn;
-        np.compact = last ? 1 : 0;
+        np.out = last && !sc ? d->hn : d->xn;
+        np.compact = last && !sc ? 1 : 0;
         if (last) {
             VXK_DCUDA(vxk::launch_add_norm(np, cs));
         } else {
@@ -676,6 +765,10 @@ void forward(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slot
         }
     }
 
+    if (sc) {
+        score_rows(d, *sc, rows, cs);
+        return;
+    }
     for (int32_t r0 = 0; r0 < n_out; r0 += vxk::kHeadRows) {
         const int32_t nr = std::min<int32_t>(vxk::kHeadRows, n_out - r0);
         float * lg = logits ? logits + (int64_t) r0 * d->vocab : nullptr;
@@ -804,6 +897,19 @@ vxk_status vxk_decoder_forward(vxk_decoder * d, const int32_t * tokens, const in
     });
 }
 
+vxk_status vxk_decoder_score(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slots, const int32_t * given,
+                             int32_t n_top, float * logprob, float * entropy, int32_t * top_ids, float * top_logprobs,
+                             void * cuda_stream) {
+    if (!d) return VXK_STATUS_INVALID_ARGUMENT;
+    return dguarded(d, [&] {
+        if (!given) dfail(VXK_STATUS_INVALID_ARGUMENT, "null argument");
+        if (n_top < 0 || n_top > vxk::kMaxTop || n_top > d->vocab)
+            dfail(VXK_STATUS_INVALID_ARGUMENT, "n_top must be in [0, min(16, vocab)]");
+        const ScoreCall sc{given, n_top, logprob, entropy, top_ids, top_logprobs};
+        forward(d, tokens, audio_slots, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(cuda_stream), &sc);
+    });
+}
+
 vxk_status vxk_decoder_write_enc(vxk_decoder * d, int32_t stream, int64_t frame, int32_t n, const float * rows,
                                  void * cuda_stream) {
     if (!d) return VXK_STATUS_INVALID_ARGUMENT;
@@ -899,6 +1005,10 @@ vxk_status vxk_decoder_sync(vxk_decoder * d, void * cuda_stream, int32_t timeout
     if (st != VXK_STATUS_OK) return st;
     st = vxk_head_sync(d->head, cuda_stream, timeout_ms);
     if (st != VXK_STATUS_OK) d->last_error = "head reported a device error";
+    if (st == VXK_STATUS_OK && d->prompt) {
+        st = vxk_prompt_sync(d->prompt, cuda_stream, timeout_ms);
+        if (st != VXK_STATUS_OK) d->last_error = "packed attention reported a device error";
+    }
     return st;
 }
 

@@ -15,6 +15,7 @@
 struct vxk_qweight;
 struct vxk_pool;
 struct vxk_enc_pool;
+struct vxk_prompt;
 
 namespace vxk {
 
@@ -355,6 +356,12 @@ struct PromptAttnParams {
     int32_t * error;
 };
 
+// vxk_prompt_rope with the angles of another table of `table_rows` positions (the cache's
+// own, so that a row rotates here as it does there); 0 or a vxk_status number.
+int32_t prompt_rope_with(vxk_prompt * prompt, const float2 * table, int32_t table_rows, const float * q, const float * k,
+                         const float * v, void * q16, void * k16, void * v16, cudaStream_t stream);
+// n 16-bit values to fp32.
+cudaError_t launch_widen(const void * in, float * out, int64_t n, int32_t dtype, cudaStream_t stream);
 cudaError_t launch_rope_table(float2 * table, int32_t rows, int32_t head_dim, double log_theta, cudaStream_t stream);
 cudaError_t launch_prompt_rope(const PromptRopeParams & p, cudaStream_t stream);
 // Tensor maps {head_dim, heads, rows} with boxes of 64 dims: tmq {64, heads of a tile,
@@ -522,6 +529,8 @@ struct PoolShape {
     float rope_theta;
 };
 PoolShape pool_shape(const vxk_pool * pool);
+// The pool's RoPE table, [rows][head_dim / 2] (cos, sin) on its device.
+const float2 * pool_rope_table(const vxk_pool * pool, int32_t * rows);
 // True when pool_decode_layer_quant applies (an f16 cache, 4 query heads of
 // 128 dims per kv head).
 bool pool_decode_quant_ok(const vxk_pool * pool);

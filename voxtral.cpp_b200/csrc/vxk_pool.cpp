@@ -639,6 +639,11 @@ PoolShape pool_shape(const vxk_pool * pool) {
                      c.rope_theta};
 }
 
+const float2 * pool_rope_table(const vxk_pool * pool, int32_t * rows) {
+    *rows = pool->cfg.max_position;
+    return pool->d_rope;
+}
+
 bool pool_decode_quant_ok(const vxk_pool * pool) {
     return pool && pool->cfg.dtype == VXK_DTYPE_F16 && pool->cfg.head_dim == kHeadDim &&
            pool->cfg.n_q_heads == pool->cfg.n_kv_heads * kGroup;

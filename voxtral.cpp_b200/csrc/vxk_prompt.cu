@@ -19,6 +19,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
+template <int DT>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if constexpr (DT == 30) {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    } else {
+        return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    }
+}
+
 // (cos, sin) of position * theta^(-2i / head_dim), in 64 bits: at position 10^5 a
 // 32-bit angle is off by 4e-3 of a radian, more than a 16-bit value resolves.
 __global__ void rope_table_kernel(float2 * table, int64_t n, int32_t half, double log_theta) {
@@ -76,7 +85,29 @@ __global__ void __launch_bounds__(256) rope_kernel(const PromptRopeParams p) {
     }
 }
 
+// Eight values a thread.
+template <int DT>
+__global__ void __launch_bounds__(256) widen_kernel(const uint4 * in, float4 * out, int64_t n8) {
+    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (i >= n8) return;
+    const uint4 u = in[i];
+    const float2 a = unpack2<DT>(u.x), b = unpack2<DT>(u.y), c = unpack2<DT>(u.z), d = unpack2<DT>(u.w);
+    out[2 * i] = make_float4(a.x, a.y, b.x, b.y);
+    out[2 * i + 1] = make_float4(c.x, c.y, d.x, d.y);
+}
+
 }  // namespace
+
+cudaError_t launch_widen(const void * in, float * out, int64_t n, int32_t dtype, cudaStream_t stream) {
+    const int64_t n8 = n / 8;
+    const unsigned grid = (unsigned) ((n8 + 255) / 256);
+    if (dtype == 30) {
+        widen_kernel<30><<<grid, 256, 0, stream>>>(static_cast<const uint4 *>(in), reinterpret_cast<float4 *>(out), n8);
+    } else {
+        widen_kernel<1><<<grid, 256, 0, stream>>>(static_cast<const uint4 *>(in), reinterpret_cast<float4 *>(out), n8);
+    }
+    return cudaGetLastError();
+}
 
 cudaError_t launch_rope_table(float2 * table, int32_t rows, int32_t head_dim, double log_theta, cudaStream_t stream) {
     const int64_t n = (int64_t) rows * (head_dim / 2);

@@ -98,6 +98,7 @@ struct vxk_prompt {
     cudaEvent_t ev_sync = nullptr;
     int sm_count = 0;
     int32_t rows = -1;          // rows of the current plan, -1 before the first
+    int64_t last_position = -1; // the largest of its positions
     std::string last_error;
 };
 
@@ -168,7 +169,43 @@ void check_buffers(const vxk_prompt * p, std::initializer_list<const void *> ptr
     }
 }
 
+void rope(vxk_prompt * prompt, const float2 * table, const float * q, const float * k, const float * v, void * q16,
+          void * k16, void * v16, cudaStream_t cs) {
+    const vxk_prompt_config & c = prompt->cfg;
+    check_buffers(prompt, {q, k, v, q16, k16, v16});
+    if (prompt->rows == 0) return;
+    PromptDevice scope(c.device);
+    vxk::PromptRopeParams a{};
+    a.plan = prompt->d_plan;
+    a.table = table;
+    a.rows = prompt->rows;
+    a.n_q = c.n_q_heads;
+    a.n_kv = c.n_kv_heads;
+    a.head_dim = c.head_dim;
+    a.dtype = (int32_t) c.dtype;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q16 = static_cast<uint16_t *>(q16);
+    a.k16 = static_cast<uint16_t *>(k16);
+    a.v16 = static_cast<uint16_t *>(v16);
+    a.error = prompt->d_error;
+    VXK_PCUDA(vxk::launch_prompt_rope(a, cs));
+}
+
 }  // namespace
+
+namespace vxk {
+
+int32_t prompt_rope_with(vxk_prompt * prompt, const float2 * table, int32_t table_rows, const float * q, const float * k,
+                         const float * v, void * q16, void * k16, void * v16, cudaStream_t stream) {
+    return pguarded(prompt, [&] {
+        if (prompt->last_position >= table_rows) pfail(VXK_STATUS_INVALID_ARGUMENT, "a position lies behind the table");
+        rope(prompt, table, q, k, v, q16, k16, v16, stream);
+    });
+}
+
+}  // namespace vxk
 
 extern "C" {
 
@@ -258,14 +295,16 @@ vxk_status vxk_prompt_plan(vxk_prompt * prompt, const int32_t * n_rows, const in
         const vxk_prompt_config & c = prompt->cfg;
         if (!n_rows || n_seqs < 1 || n_seqs > c.max_seqs)
             pfail(VXK_STATUS_INVALID_ARGUMENT, "n_seqs must be in [1, max_seqs]");
-        int64_t total = 0;
+        int64_t total = 0, furthest = -1;
         for (int32_t i = 0; i < n_seqs; ++i) {
             const int64_t first = first_position ? first_position[i] : 0;
             if (n_rows[i] < 0 || first < 0) pfail(VXK_STATUS_INVALID_ARGUMENT, "negative rows or position");
             if (c.max_position > 0 && n_rows[i] > 0 && first + n_rows[i] > c.max_position)
                 pfail(VXK_STATUS_INVALID_ARGUMENT, "a position reaches max_position");
+            if (n_rows[i] > 0) furthest = std::max(furthest, first + n_rows[i] - 1);
             total += n_rows[i];
         }
+        if (furthest > INT32_MAX) pfail(VXK_STATUS_INVALID_ARGUMENT, "a position does not fit 32 bits");
         if (total > c.max_rows) pfail(VXK_STATUS_INVALID_ARGUMENT, "the plan has more than max_rows rows");
         PromptDevice scope(c.device);
         cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
@@ -322,6 +361,7 @@ vxk_status vxk_prompt_plan(vxk_prompt * prompt, const int32_t * n_rows, const in
         VXK_PCUDA(cudaEventRecord(prompt->plan_ev[slot], cs));
         prompt->plan_next ^= 1;
         prompt->rows = (int32_t) total;
+        prompt->last_position = furthest;
     });
 }
 
@@ -336,27 +376,8 @@ vxk_status vxk_prompt_rope(vxk_prompt * prompt, const float * q, const float * k
                            void * k16, void * v16, void * cuda_stream) {
     if (!prompt) return VXK_STATUS_INVALID_ARGUMENT;
     return pguarded(prompt, [&] {
-        const vxk_prompt_config & c = prompt->cfg;
-        if (c.max_position == 0) pfail(VXK_STATUS_INVALID_STATE, "the prompt was created without positions");
-        check_buffers(prompt, {q, k, v, q16, k16, v16});
-        if (prompt->rows == 0) return;
-        PromptDevice scope(c.device);
-        vxk::PromptRopeParams a{};
-        a.plan = prompt->d_plan;
-        a.table = prompt->table;
-        a.rows = prompt->rows;
-        a.n_q = c.n_q_heads;
-        a.n_kv = c.n_kv_heads;
-        a.head_dim = c.head_dim;
-        a.dtype = (int32_t) c.dtype;
-        a.q = q;
-        a.k = k;
-        a.v = v;
-        a.q16 = static_cast<uint16_t *>(q16);
-        a.k16 = static_cast<uint16_t *>(k16);
-        a.v16 = static_cast<uint16_t *>(v16);
-        a.error = prompt->d_error;
-        VXK_PCUDA(vxk::launch_prompt_rope(a, static_cast<cudaStream_t>(cuda_stream)));
+        if (prompt->cfg.max_position == 0) pfail(VXK_STATUS_INVALID_STATE, "the prompt was created without positions");
+        rope(prompt, prompt->table, q, k, v, q16, k16, v16, static_cast<cudaStream_t>(cuda_stream));
     });
 }
 

@@ -237,6 +237,7 @@ SIGNATURES = {
     "vxk_decoder_last_error": (_I32, [_P, C.c_char_p, C.c_size_t]),
     "vxk_decoder_get_info": (_I32, [_P, C.POINTER(DecoderInfo)]),
     "vxk_decoder_forward": (_I32, [_P, _I32P, _I32P, _P, _P, _P, _P]),
+    "vxk_decoder_score": (_I32, [_P, _I32P, _I32P, _I32P, _I32, _P, _P, _P, _P, _P]),
     "vxk_decoder_write_enc": (_I32, [_P, _I32, _I64, _I32, _P, _P]),
     "vxk_decoder_write_audio": (_I32, [_P, _I32, _I64, _I32, _P, _P]),
     "vxk_decoder_adapt": (_I32, [_P, _I32, _I32P, _I64P, _I64P, _P]),
@@ -867,6 +868,15 @@ class Decoder:
         a = _i32_array(list(audio_slots))
         self._check(self.lib.vxk_decoder_forward(self.h, t, a, argmax_ptr, logits_ptr or None, hidden_ptr or None,
                                                  cuda_stream or None))
+
+    def score(self, tokens, audio_slots, given, n_top: int, logprob_ptr: int = 0, entropy_ptr: int = 0,
+              top_ids_ptr: int = 0, top_logprobs_ptr: int = 0, cuda_stream: int = 0):
+        """Log probabilities of given[r] (-1: not scored) behind every row of the planned batch."""
+        t, a, g = (_i32_array(list(x)) for x in (tokens, audio_slots, given))
+        if not len(t) == len(a) == len(g):
+            raise VxkError(INVALID_ARGUMENT, "tokens, audio_slots and given have one entry per row")
+        self._check(self.lib.vxk_decoder_score(self.h, t, a, g, n_top, logprob_ptr or None, entropy_ptr or None,
+                                               top_ids_ptr or None, top_logprobs_ptr or None, cuda_stream or None))
 
     def write_enc(self, stream: int, frame: int, n: int, rows_ptr: int, cuda_stream: int = 0):
         self._check(self.lib.vxk_decoder_write_enc(self.h, stream, frame, n, rows_ptr, cuda_stream or None))
