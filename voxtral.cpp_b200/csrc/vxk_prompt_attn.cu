@@ -49,8 +49,7 @@ struct Shape {
     static constexpr int kOffBar = kOffRing + kStages * kTileBytes;
     // barriers
     static constexpr int kFull = 0, kEmpty = kStages, kReady = 2 * kStages, kQFull = 3 * kStages, kQEmpty = kQFull + 2,
-                         kSFull = kQEmpty + 2, kPFull = kSFull + 2, kODone = kPFull + 4, kOHalf = kODone + 2,
-                         kDrain = kOHalf + 2;
+                         kSFull = kQEmpty + 2, kPFull = kSFull + 2, kODone = kPFull + 4, kDrain = kODone + 2;
     static constexpr int kBars = kDrain + 1;
     static constexpr int kOffMisc = kOffBar + 8 * kBars;  // TMEM base, abort flag, V flags
     static constexpr int kSmem = kOffMisc + 8 + 2 * kFlags * 4 + 1024;
@@ -251,19 +250,19 @@ struct RowState {
     float sum;
 };
 
-// 64 scores of a row: the running maximum, p into TMEM at tp, the sum.  hi, lo: the
-// columns [lo, hi) of these that the row attends (MASKED).  Where some row's maximum has
-// outgrown kSlack, grown() is called before anything depends on the new one: it waits for the
-// products so far and multiplies O by its argument.
-template <int DT, bool MASKED, typename F>
-__device__ __forceinline__ bool half_step(float (&x)[64], uint32_t tp, float c, int hi, int lo, RowState & r, F && grown) {
-    bool whole[2] = {true, true}, none[2] = {false, false};
+// 128 scores of a row: the running maximum, p into TMEM at tp, the sum.  hi, lo: the columns
+// [lo, hi) that the row attends (MASKED).  Where some row's maximum has outgrown kSlack,
+// grown() multiplies O by its argument first.  half_done(k): a half of p is stored.
+template <int DT, bool MASKED, typename F, typename G>
+__device__ __forceinline__ void tile_step(float (&x)[128], uint32_t tp, float c, int hi, int lo, RowState & r, F && grown,
+                                          G && half_done) {
+    bool none[4] = {false, false, false, false};
     if constexpr (MASKED) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            whole[k] = __all_sync(0xffffffffu, hi >= 32 * k + 32 && lo <= 32 * k);
+        for (int k = 0; k < 4; ++k) {
+            const bool whole = __all_sync(0xffffffffu, hi >= 32 * k + 32 && lo <= 32 * k);
             none[k] = __all_sync(0xffffffffu, hi <= 32 * k || lo >= 32 * k + 32);
-            if (!whole[k] && !none[k]) {
+            if (!whole && !none[k]) {
 #pragma unroll
                 for (int e = 32 * k; e < 32 * k + 32; ++e)
                     if (e >= hi || e < lo) x[e] = -INFINITY;
@@ -272,7 +271,7 @@ __device__ __forceinline__ bool half_step(float (&x)[64], uint32_t tp, float c, 
     }
     float mt[4] = {r.m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 4; ++k) {
         if (MASKED && none[k]) continue;
 #pragma unroll
         for (int e = 32 * k; e < 32 * k + 32; e += 2) mt[e / 2 % 4] = max3(mt[e / 2 % 4], x[e], x[e + 1]);
@@ -283,25 +282,25 @@ __device__ __forceinline__ bool half_step(float (&x)[64], uint32_t tp, float c, 
         const float f = grow ? ex2f((r.m - mn) * c) : 1.0f;
         r.sum *= f;
         if (grow) r.m = mn;
-        if (!grown(f)) return false;
+        grown(f);
     }
     if (r.m == -INFINITY) r.m = mn;                  // nothing in O or the sum yet
     const float off = r.m == -INFINITY ? 0.0f : -r.m * c;
     const uint64_t c2 = pair(c, c), off2 = pair(off, off);
     uint64_t total[2] = {0, 0};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 4; ++k) {
         if (MASKED && none[k]) {
             const uint32_t zero[16] = {};
             tmem_store16(tp + 16 * k, zero);
         } else {
             exp_chunk<DT>(x + 32 * k, tp + 16 * k, c2, off2, total);
         }
+        if (k & 1) half_done(k >> 1);
     }
     float a, b;
     unpair(add2(total[0], total[1]), a, b);
     r.sum += a + b;
-    return true;
 }
 
 template <int DT, int HD>
@@ -342,7 +341,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             mbar_init(&bars[S::kPFull + 2 * s], 4);  // keys 0-63
             mbar_init(&bars[S::kPFull + 2 * s + 1], 4);
             mbar_init(&bars[S::kODone + s], 1);
-            mbar_init(&bars[S::kOHalf + s], 1);
         }
         mbar_init(&bars[S::kDrain], 1);
         *abort_flag = 0;
@@ -469,8 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
 #pragma unroll
                                 for (int ks = 0; ks < kTile / 32; ++ks)  // 16 keys: 8 columns of P, 2 KB of V
                                     mma_ts(d, a + 8 * ks, dv + 128 * ks, idesc_o, (j | ks) != 0);
-                                tc_commit<1>(&bars[S::kOHalf + s]);
-                            }
+                                }
                             __syncwarp();
                             bits ^= kBitP << s;  // the second half's barrier has the first's parity
                             ok = wait_bit(S::kPFull + 2 * s + 1, kBitP << s);
@@ -566,39 +563,26 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                 ok = __all_sync(0xffffffffu, tc_wait(&bars[S::kSFull + s], cs & 1, abort_flag, p.error));
                 if (!ok) break;
                 tc_fence_after();
-                float x[64];
-                tmem_load32(ts, reinterpret_cast<uint32_t *>(x));
-                tmem_load32(ts + 32, reinterpret_cast<uint32_t *>(x) + 32);
+                float x[128];
+#pragma unroll
+                for (int k = 0; k < 128; k += 32) tmem_load32(ts + k, reinterpret_cast<uint32_t *>(x) + k);
                 const int k0 = (it.lo + j) * kTile;
                 const bool masked =
                     k0 + kTile > (p.causal ? min(first + 1, it.len) : it.len) || (p.window > 0 && last - p.window >= k0);
                 const int hi = (p.causal ? min(token + 1, it.len) : it.len) - k0;
                 const int lo = p.window > 0 ? token - p.window + 1 - k0 : 0;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    tmem_wait_ld();
-                    // O is complete up to the last tile when S is there, and up to this tile's
-                    // first half when that is said to be
-                    auto grown = [&](float f) {
-                        if (half && !__all_sync(0xffffffffu, tc_wait(&bars[S::kOHalf + s], cs & 1, abort_flag, p.error)))
-                            return false;
-                        tc_fence_after();
-                        if (j + half > 0) scale_o<HD>(to, f);
-                        return true;
-                    };
-                    ok = masked ? half_step<DT, true>(x, ts + 32 * half, c, hi - 64 * half, lo - 64 * half, row, grown)
-                                : half_step<DT, false>(x, ts + 32 * half, c, 0, 0, row, grown);
-                    if (!ok) break;
+                tmem_wait_ld();
+                auto grown = [&](float f) {  // O is complete up to the last tile when S is there
+                    if (j > 0) scale_o<HD>(to, f);
+                };
+                auto half_done = [&](int half) {
                     tmem_wait_st();
-                    if (half == 0) {  // under way while the first half is handed over
-                        tmem_load32(ts + 64, reinterpret_cast<uint32_t *>(x));
-                        tmem_load32(ts + 96, reinterpret_cast<uint32_t *>(x) + 32);
-                    }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars[S::kPFull + 2 * s + half]);
-                }
-                if (!ok) break;
+                };
+                if (masked) tile_step<DT, true>(x, ts, c, hi, lo, row, grown, half_done);
+                else tile_step<DT, false>(x, ts, c, 0, 0, row, grown, half_done);
             }
             if (!ok) break;
             // epilogue: O / sum
