@@ -13,13 +13,13 @@
 // takes 16 elements of each and their maximum first, so that the sums are rescaled at
 // most once a strip.
 //
-// The top list is found by comparing with a lower bound of its end and collecting the few
-// keys that reach it in shared memory.  In a run's first strip every warp takes the
-// n_top-th largest of its lanes' maxima, which is no more than the n_top-th largest of
-// all; after that strip, the fourth and every sixteenth (t strips bring about n_top keys
-// above the bound of the t before them) the keys are ranked against each other, all at
-// once, and the list's end becomes the bound.  Keys that do not fit (equal or rising logits) send their strips
-// through a slower bound of which at most n_top groups of 64 elements can be above.
+// The top list costs the scan nothing but each thread's running maximum, noted a dozen
+// times a run.  Behind the run the n_top-th largest of 64 groups' maxima bounds the
+// list's end from below; the few noted maxima that reach it name the elements to read
+// again (from L2), and the keys found there are ranked against each other, all at once.
+// Where too many reach the bound (rows of equal or masked logits) the run's strips are
+// gone through once more in order, each with a bound that at most n_top groups of 64
+// elements reach.
 #include "vxk_internal.h"
 #include "vxk_score.h"
 #include "vxk_tc.h"
@@ -184,20 +184,21 @@ __global__ void __launch_bounds__(kThreads, 2) score_warp_kernel(const ScoreLogi
     finish<DT>(p, row, warp_join(a), top.key);
 }
 
-constexpr int kKeys = 2304;    // collected keys of a run: 8 warps x 16 lanes x 16, and ragged ends
-constexpr int kStages = 4;     // strips of a CTA under way or being read
-// The list's code needs more registers than three CTAs of an SM leave.
-constexpr int ctas_per_sm(bool list) { return list ? 2 : kScoreCtasPerSm; }
-constexpr int kSpare = 8;      // keys beyond n_top that are let be
-constexpr int kLook = 16;      // most strips between two looks at their number
+constexpr int kStages = 3;     // strips of a CTA under way or being read
+constexpr int kNotes = 12;     // maxima that a thread notes in a run
+constexpr int kCands = 512;    // noted maxima that reach the bound
+// keys at once: those of n_top groups of 64 elements, the list, and a row's ragged ends
+constexpr int kKeys = kMaxTop * 64 + kMaxTop + 16;
 
 struct Collected {
     unsigned long long key[kKeys];
     unsigned long long best[kMaxTop];
     unsigned long long group[kThreads];
     unsigned long long bound;  // a key that bounds the list's end from below
-    uint32_t warm;             // the upper half of one (any key of that value may belong to the list)
     int count;
+    int n_cands;
+    uint16_t cand[kCands];     // thread + 256 x note
+    float note[kNotes][kThreads];
 };
 
 // Ranks `n` collected keys (all threads; n is the same for all): the n_top largest, in
@@ -225,53 +226,15 @@ __device__ __forceinline__ void rank_kept(Collected & c, int n_top) {
     rank_keys(c, n, n_top);
 }
 
-// What the bound leaves in question is above this.
-__device__ __forceinline__ float below_bound(const Collected & c) {
-    return top_below(max((uint32_t) (c.bound >> 32), c.warm));
+// Appends a key; one that finds no room is only counted.
+__device__ __forceinline__ void append(Collected & c, unsigned long long k) {
+    const int place = atomicAdd(&c.count, 1);
+    if (place < kKeys) c.key[place] = k;
 }
 
-// Appends a thread's keys of a strip that reach the bound (low: below_bound, or an older
-// one's); returns whether many are there.
-template <int DT>
-__device__ __forceinline__ bool collect(Collected & c, const Row<DT> & r, int v0, const float (&x)[Elem<DT>::kPer],
-                                        float m, float low, int n_top) {
-    using E = Elem<DT>;
-    if (v0 >= r.n_vec || m <= low) return false;
-    const unsigned long long bound = max(c.bound, (unsigned long long) c.warm << 32);
-    bool many = false;
-#pragma unroll
-    for (int j = 0; j < E::kLoads; ++j) {
-        if (v0 + j * kThreads >= r.n_vec) break;
-#pragma unroll
-        for (int i = 0; i < E::kVec; ++i) {
-            const float v = x[j * E::kVec + i];
-            if (!(v <= low)) {
-                const unsigned long long k = top_key(v, r.lead + (v0 + j * kThreads) * E::kVec + i);
-                if (k >= bound) {
-                    const int place = atomicAdd(&c.count, 1);
-                    if (place < kKeys) c.key[place] = k;
-                    many |= place >= n_top + kSpare;
-                }
-            }
-        }
-    }
-    return many;
-}
-
-// A strip whose keys may not fit: its own bound first, then its keys, behind the `before`
-// keys of earlier strips (the same number in all threads).
-template <int DT>
-__device__ __forceinline__ void collect_first(Collected & c, const Row<DT> & r, int v0, const float (&x)[Elem<DT>::kPer],
-                                              float m, int before, int n_top) {
-    using E = Elem<DT>;
-    int at = -1;  // the lowest index of the thread's largest element
-#pragma unroll
-    for (int j = E::kLoads - 1; j >= 0; --j)
-#pragma unroll
-        for (int i = E::kVec - 1; i >= 0; --i)
-            if (v0 + j * kThreads < r.n_vec && top_bits(x[j * E::kVec + i]) == top_bits(m))
-                at = r.lead + (int) (v0 + j * kThreads) * E::kVec + i;
-    const unsigned long long mine = v0 < r.n_vec ? top_key(m, at) : 0ull;
+// The n_top-th largest of the 64 groups' keys, of four threads each with its own largest
+// (0: none), into c.bound where it is more.  Ends in front of a barrier.
+__device__ __forceinline__ void group_bound(Collected & c, unsigned long long mine, int n_top) {
     unsigned long long g = max(mine, __shfl_xor_sync(kAll, mine, 1));
     g = max(g, __shfl_xor_sync(kAll, g, 2));
     if (threadIdx.x % 4 == 0) c.group[threadIdx.x / 4] = g;
@@ -282,14 +245,97 @@ __device__ __forceinline__ void collect_first(Collected & c, const Row<DT> & r, 
         for (int j = 0; j < kThreads / 4; ++j) above += c.group[j] > k;
         if (above == n_top - 1 && k > c.bound) c.bound = k;  // keys differ: one thread
     }
-    if (threadIdx.x == 0) c.count = before;
+}
+
+// The run's list (strips [c0, c1) of row r) behind its scan: c.key[0 .. n_top) on return.
+// `ragged` keys are in c.key already; `most` is the thread's largest element, its maxima of
+// every `span` strips are noted.
+template <int DT>
+__device__ __forceinline__ void select(Collected & c, const Row<DT> & r, int c0, int c1, int span, float most, int ragged,
+                                       int n_top) {
+    using E = Elem<DT>;
+    constexpr int kStep = kThreads * E::kLoads;
+    const int tid = threadIdx.x;
+    // maxima as keys: the value, and who holds it
+    const uint32_t bits = c0 * kStep + tid < r.n_vec ? top_bits(most) : 0u;
+    if (tid == 0) {
+        c.bound = 0ull;
+        c.n_cands = 0;
+    }
+    group_bound(c, bits ? top_key(most, tid) : 0ull, n_top);
     __syncthreads();
-    collect(c, r, v0, x, m, below_bound(c), n_top);
+    const float low = top_below((uint32_t) (c.bound >> 32));
+    for (int e = 0; e * span < c1 - c0; ++e) {
+        if ((c0 + e * span) * kStep + tid < r.n_vec && !(c.note[e][tid] <= low)) {
+            const int place = atomicAdd(&c.n_cands, 1);
+            if (place < kCands) c.cand[place] = (uint16_t) (tid + 256 * e);
+        }
+    }
     __syncthreads();
+    const int n_cands = c.n_cands;
+    if (n_cands <= kCands) {
+        for (int i = tid; i < n_cands * span * E::kLoads; i += kThreads) {
+            const int who = c.cand[i / (span * E::kLoads)], in = i % (span * E::kLoads);
+            const int strip = c0 + who / 256 * span + in / E::kLoads;
+            const int v = strip * kStep + in % E::kLoads * kThreads + who % 256;
+            if (strip >= c1 || v >= r.n_vec) continue;
+            float x[E::kVec];
+            unpack<DT>(load_stream(r.body + (int64_t) v * 16), x);
+#pragma unroll
+            for (int j = 0; j < E::kVec; ++j)
+                if (!(x[j] <= low)) append(c, top_key(x[j], r.lead + v * E::kVec + j));
+        }
+    }
+    __syncthreads();
+    const int n = c.count;
+    __syncthreads();
+    // (fewer than n_top where the rest is NaN)
+    if (n_cands <= kCands && n <= kKeys && n >= min(n_top, (c1 - c0) * kStep * E::kVec)) {
+        rank_keys(c, n, n_top);
+        return;
+    }
+    if (tid == 0) {
+        c.bound = 0ull;
+        c.count = ragged;
+    }
+    __syncthreads();
+    for (int s = c0; s < c1; ++s) {
+        const int v0 = s * kStep + tid;
+        float x[E::kPer];
+        take_strip<DT, false>(r, r.body + (int64_t) v0 * 16, v0, kThreads, x);
+        // A later element of the list's last value stands behind it.
+        const uint32_t last = (uint32_t) (c.bound >> 32);
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < E::kPer; ++i) any |= v0 + i / E::kVec * kThreads < r.n_vec && top_bits(x[i]) > last;
+        if (!__syncthreads_or(any)) continue;
+        int at = -1;  // the thread's first element of the largest bits
+        uint32_t largest = 0;
+#pragma unroll
+        for (int i = 0; i < E::kPer; ++i) {
+            const int v = v0 + i / E::kVec * kThreads;
+            if (v < r.n_vec && top_bits(x[i]) > largest) {
+                largest = top_bits(x[i]);
+                at = r.lead + v * E::kVec + i % E::kVec;
+            }
+        }
+        group_bound(c, largest ? ((unsigned long long) largest << 32) | (0xFFFFFFFFu - (uint32_t) at) : 0ull, n_top);
+        __syncthreads();
+        const unsigned long long bound = c.bound;
+#pragma unroll
+        for (int i = 0; i < E::kPer; ++i) {
+            const int v = v0 + i / E::kVec * kThreads;
+            const unsigned long long k = top_key(x[i], r.lead + v * E::kVec + i % E::kVec);
+            if (v < r.n_vec && k >= bound) append(c, k);
+        }
+        __syncthreads();
+        rank_kept(c, n_top);
+    }
+    rank_kept(c, n_top);
 }
 
 template <int DT, bool LIST>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(LIST)) score_block_kernel(const ScoreLogitsParams p) {
+__global__ void __launch_bounds__(kThreads, kScoreCtasPerSm) score_block_kernel(const ScoreLogitsParams p) {
     using E = Elem<DT>;
     __shared__ Stat stats[kWarps];
     __shared__ Collected keys;
@@ -348,7 +394,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(LIST)) score_block_kerne
         Stat a = stat_empty();
         if (tid == 0) {
             keys.bound = 0ull;
-            keys.warm = 0u;
             keys.count = 0;
         }
         __syncthreads();
@@ -364,9 +409,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(LIST)) score_block_kerne
         }
         const int ragged = keys.count;
         __syncthreads();
-        bool many = false;
-        float low = __uint_as_float(0x7fc00000u);
-        int since = c0;                  // first strip since the last look
+        const int span = (c1 - c0 + kNotes - 1) / kNotes;  // strips of a note
+        float most = -INFINITY, note = -INFINITY;
+        int noted = 0, left = span;
         for (int c = c0; c < c1; ++c) {
             const int v0 = c * kStep + tid;
             float x[E::kPer];
@@ -379,64 +424,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(LIST)) score_block_kerne
             feed(turn + kStages - 2);
             add_strip(a, x, m);
             if constexpr (LIST) {
-                if (c == c0) {
-                    // the n_top-th largest of the lanes' maxima
-                    uint32_t largest = v0 < r.n_vec ? top_bits(m) : 0u, v = 0;
-                    for (int i = 0; i < n_top; ++i) {
-                        v = __reduce_max_sync(kAll, largest);
-                        const unsigned who = __ballot_sync(kAll, largest == v);
-                        if (lane == __ffs(who) - 1) largest = 0u;
-                    }
-                    if (lane == 0) atomicMax(&keys.warm, v);  // 0: fewer lanes than places
-                    __syncwarp();
-                    low = below_bound(keys);
-                }
-                many |= collect(keys, r, v0, x, m, low, n_top);
-                const int seen = c - c0 + 1;
-                if (seen == 1 || seen == 4 || seen % kLook == 0 || c + 1 == c1) {
-                    if (__syncthreads_or(many)) {
-                        many = false;
-                        if (keys.count > kKeys) {
-                            // they did not fit: back to those of the strips before the last look
-                            // (at most n_top + kSpare, or they would have been ranked), then the
-                            // strips since, one by one
-                            __syncthreads();
-                            if (tid == 0) {
-                                const int64_t lo = r.lead + (int64_t) since * kStep * E::kVec;
-                                const int64_t hi =
-                                    r.lead + min((int64_t) (c + 1) * kStep, (int64_t) r.n_vec) * E::kVec;
-                                int n = 0;
-                                for (int i = 0; i < max(n_top + kSpare, ragged); ++i) {
-                                    const unsigned long long k = keys.key[i];
-                                    if (top_index(k) < lo || top_index(k) >= hi) keys.key[n++] = k;
-                                }
-                                keys.count = n;
-                            }
-                            __syncthreads();
-                            for (int again = since; again <= c; ++again) {
-                                const int before = keys.count;
-                                __syncthreads();
-                                const int w0 = again * kStep + tid;
-                                const float most =
-                                    take_strip<DT, false>(r, r.body + (int64_t) w0 * 16, w0, kThreads, x);
-                                collect_first(keys, r, w0, x, most, before, n_top);
-                                rank_kept(keys, n_top);
-                            }
-                        } else {
-                            rank_kept(keys, n_top);
-                        }
-                    }
-                    since = c + 1;
-                    low = below_bound(keys);
+                note = fmaxf(note, m);
+                if (--left == 0 || c + 1 == c1) {
+                    keys.note[noted++][tid] = note;
+                    most = fmaxf(most, note);
+                    note = -INFINITY;
+                    left = span;
                 }
             }
         }
         a = warp_join(a);
         if (lane == 0) stats[warp] = a;
         __syncthreads();
-        if (n_top) {
-            rank_kept(keys, n_top);
-        }
+        if (n_top) select(keys, r, c0, c1, span, most, ragged, n_top);
         if (warp == 0) {
             a = lane < kWarps ? stats[lane] : stat_empty();
             a = warp_join(a);
@@ -470,7 +470,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(LIST)) score_block_kerne
                 // the n_top-th largest of the parts' largest keys bounds the list from below
                 if (tid == 0) {
                     keys.bound = 0ull;
-                    keys.warm = 0u;
                     keys.count = 0;
                 }
                 Stat one = stat_empty();
@@ -526,7 +525,7 @@ cudaError_t launch(ScoreLogitsParams & p, int sms, cudaStream_t stream) {
     }
     const int64_t n_vec = p.out.vocab / Elem<DT>::kVec;
     p.strips = (n_vec + kThreads * Elem<DT>::kLoads - 1) / (kThreads * Elem<DT>::kLoads);
-    const int64_t grid = std::min<int64_t>(p.strips * p.rows, (int64_t) sms * ctas_per_sm(p.out.n_top > 0));
+    const int64_t grid = std::min<int64_t>(p.strips * p.rows, (int64_t) sms * kScoreCtasPerSm);
     constexpr int kRing = kStages * kThreads * Elem<DT>::kLoads * 16;
     auto kernel = p.out.n_top > 0 ? score_block_kernel<DT, true> : score_block_kernel<DT, false>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
