@@ -95,7 +95,7 @@ def check(got, l64, tokens, n_top):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("rows,vocab,pad,n_top", [
     (1, 1, 0, 1), (3, 7, 1, 5), (2, 33, 0, 16), (19, 511, 3, 1), (5, 4096, 0, 8), (9, 4097, 5, 16), (1, 131072, 0, 16),
-    (3, 131071, 0, 4), (301, 12289, 2, 3), (700, 40, 7, 2), (64, 32003, 0, 0)])
+    (3, 131071, 0, 4), (301, 12289, 2, 3), (700, 40, 7, 2), (64, 32003, 0, 0), (2, 300007, 1, 16)])
 def test_logits_match_the_definition(vxk, dtype, rows, vocab, pad, n_top):
     import torch
 
@@ -379,3 +379,33 @@ def test_hidden_rows_with_equal_logits(vxk):
         lp, ent, ids, top = run_head(vxk, w, x, np.arange(rows), n_top, F16)
         assert np.array_equal(ids[::3], np.tile(np.arange(n_top), (len(ids[::3]), 1)))
         assert np.allclose(lp[::3], -np.log(vocab), rtol=1e-6) and np.allclose(ent[::3], np.log(vocab), rtol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("n_top", [2, 5, 16])
+def test_lists_of_a_masked_vocabulary(vxk, dtype, n_top):
+    """Rows with few logits left: the list goes on with the lowest of the masked indices."""
+    import torch
+
+    vocab = 70001
+    l = torch.full((4, vocab), -float("inf"), device="cuda")
+    l[0, [3, 40000, 69999]] = torch.tensor([1.0, 3.0, 2.0], device="cuda")
+    l[1, 65536] = 0.0
+    l[2, 20000:20012] = torch.arange(12, device="cuda", dtype=torch.float32)
+    l[3, ::4099] = 1.5
+    tokens = np.array([3, 65536, 20011, 4099])
+    l = l.to(_torch_type(dtype))
+    check(score_logits(vxk, l, vocab, tokens, n_top), l.double().cpu().numpy(), tokens, n_top)
+
+
+def test_rows_with_hardly_a_number(vxk):
+    """NaN nearly everywhere: NaN outputs, and a list of indices that differ."""
+    import torch
+
+    vocab = 30000
+    l = torch.full((2, vocab), float("nan"), device="cuda")
+    l[0, 29999] = 1.0
+    lp, ent, ids, _ = score_logits(vxk, l, vocab, np.array([5, 5]), 6)
+    assert np.all(np.isnan(lp)) and np.all(np.isnan(ent)) and ids[0, 0] == 29999
+    for r in range(2):
+        assert len(set(ids[r])) == 6 and ids[r].min() >= 0 and ids[r].max() < vocab

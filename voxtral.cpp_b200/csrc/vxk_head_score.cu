@@ -427,6 +427,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) head_join_kernel(const HeadSc
     top.clear(p.n_top);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= p.n_rows) return;  // a whole warp, and only where warps do not meet
+    const int32_t token = out.tokens ? out.tokens[row] : -1;
+    const float token_logit = p.token_logits[row];
     if (p.n_top) top.raise(p.row_low[row]);
     for (int i0 = WARPS == 1 ? 0 : warp * 32; i0 < 2 * p.n_groups; i0 += WARPS * 32) {
         const int i = i0 + lane;
@@ -459,8 +461,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) head_join_kernel(const HeadSc
         for (int i = p.n_top; i < kJoinWarps * p.n_top; i += 32)  // the warp's own list is in place
             top.offer(i + lane < kJoinWarps * p.n_top ? lists[i + lane] : 0ull);
     }
-    const int32_t token = out.tokens ? out.tokens[row] : -1;
-    score_write(out, row, a, top.key, token, token >= 0 && token < out.vocab ? p.token_logits[row] : 0.0f);
+    score_write(out, row, a, top.key, token, token_logit);
 }
 
 template <int DT, int CG, int LIST>

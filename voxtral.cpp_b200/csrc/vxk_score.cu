@@ -134,13 +134,18 @@ __device__ __forceinline__ Stat warp_join(Stat a) {
     return a;
 }
 
+// A row's given token and its logit, read ahead of the row: one behind the other they take
+// longer than a small row does.
+struct Given {
+    int32_t token;
+    float logit;
+};
 template <int DT>
-__device__ __forceinline__ void finish(const ScoreLogitsParams & p, int64_t row, const Stat & a,
-                                       unsigned long long key) {
-    const int32_t token = p.out.tokens ? p.out.tokens[row] : -1;
+__device__ __forceinline__ Given given_of(const ScoreLogitsParams & p, int64_t row) {
+    Given g = {p.out.tokens ? p.out.tokens[row] : -1, 0.0f};
     const uint8_t * at = static_cast<const uint8_t *>(p.logits) + row * p.ld * Elem<DT>::kBytes;
-    const float l = token >= 0 && token < p.out.vocab ? logit_at<DT>(at, token) : 0.0f;
-    score_write(p.out, row, a, key, token, l);
+    if (g.token >= 0 && g.token < p.out.vocab) g.logit = logit_at<DT>(at, g.token);
+    return g;
 }
 
 // A row of at most one strip by one warp, its list in the warp's lanes.
@@ -151,6 +156,7 @@ __global__ void __launch_bounds__(kThreads, 2) score_warp_kernel(const ScoreLogi
     const int lane = threadIdx.x & 31;
     if (row >= p.rows) return;
     const Row<DT> r(p, row);
+    const Given given = given_of<DT>(p, row);
     Stat a = stat_empty();
     WarpTop top;
     top.clear(p.out.n_top);
@@ -181,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 2) score_warp_kernel(const ScoreLogi
         }
         add_strip(a, x, m);
     }
-    finish<DT>(p, row, warp_join(a), top.key);
+    score_write(p.out, row, warp_join(a), top.key, given.token, given.logit);
 }
 
 constexpr int kStages = 3;     // strips of a CTA under way or being read
@@ -391,6 +397,8 @@ __global__ void __launch_bounds__(kThreads, kScoreCtasPerSm) score_block_kernel(
         const int64_t row = at / strips;
         const int c0 = (int) (at - row * strips), c1 = (int) min((int64_t) strips, c0 + end - at);
         const Row<DT> r(p, row);
+        Given given = {-1, 0.0f};
+        if (warp == 0) given = given_of<DT>(p, row);
         Stat a = stat_empty();
         if (tid == 0) {
             keys.bound = 0ull;
@@ -443,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, kScoreCtasPerSm) score_block_kernel(
         }
         const unsigned long long mine = tid < n_top ? keys.key[tid] : 0ull;
         if (c1 - c0 == strips) {
-            if (warp == 0) finish<DT>(p, row, a, mine);
+            if (warp == 0) score_write(p.out, row, a, mine, given.token, given.logit);
         } else {
             // the CTAs whose runs hold this row's first and last strips
             const int64_t r0 = row * strips;
@@ -508,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, kScoreCtasPerSm) score_block_kernel(
                 if (warp == 0) {
                     one = warp_join(lane < kWarps ? stats[lane] : stat_empty());
                     if (lane == 0) p.counters[from] = 0;
-                    finish<DT>(p, row, one, lane < n_top ? keys.key[lane] : 0ull);
+                    score_write(p.out, row, one, lane < n_top ? keys.key[lane] : 0ull, given.token, given.logit);
                 }
             }
         }
