@@ -40,6 +40,7 @@ namespace vxk {
 namespace {
 
 constexpr int kThreads = 384;
+constexpr int kMostGroups = 160;                // CTAs that share a row tile, at most
 // Registers a thread after the split: 128 x 40 + 256 x 232 = 128 x 24 + 256 x 240 = 384 x 168,
 // the launch's; which of the two leaves no role spilling goes by the list.
 template <int LIST>
@@ -412,29 +413,27 @@ __global__ void __launch_bounds__(256) head_round_kernel(const float4 * x, uint2
     }
 }
 
-// Joins the parts of a row, a lane one part at a time: by the eight warps of a CTA
-// where a row has many parts (few rows), by one warp otherwise.
+__device__ __forceinline__ int64_t part_slot(const HeadScoreParams & p, int cg, int row, int i) {
+    const int64_t unit = (int64_t) (i >> 1) * p.n_row_tiles + row / (128 * cg);
+    return (unit * cg + row / 128 % cg) * 2 + (i & 1);
+}
+
+// Joins the parts of a row by a warp, a lane one part at a time: rows with few parts.
 constexpr int kJoinWarps = 8;
-template <int WARPS>
-__global__ void __launch_bounds__(kJoinWarps * 32) head_join_kernel(const HeadScoreParams p, const ScoreOut out, int cg) {
-    __shared__ Stat stats[kJoinWarps];
-    __shared__ unsigned long long lists[kJoinWarps * kMaxTop];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = WARPS == 1 ? (int) blockIdx.x * kJoinWarps + warp : (int) blockIdx.x;
-    const int row_tile = row / (128 * cg), rank = row / 128 % cg, place = row % 128;
+__global__ void __launch_bounds__(kJoinWarps * 32) head_join_warp_kernel(const HeadScoreParams p, const ScoreOut out, int cg) {
+    const int lane = threadIdx.x & 31, row = (int) blockIdx.x * kJoinWarps + (threadIdx.x >> 5), place = row % 128;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (row >= p.n_rows) return;
+    const int32_t token = out.tokens ? out.tokens[row] : -1;
+    const float token_logit = p.token_logits[row];
     Stat a = stat_empty();
     WarpTop top;
     top.clear(p.n_top);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (row >= p.n_rows) return;  // a whole warp, and only where warps do not meet
-    const int32_t token = out.tokens ? out.tokens[row] : -1;
-    const float token_logit = p.token_logits[row];
     if (p.n_top) top.raise(p.row_low[row]);
-    for (int i0 = WARPS == 1 ? 0 : warp * 32; i0 < 2 * p.n_groups; i0 += WARPS * 32) {
+    for (int i0 = 0; i0 < 2 * p.n_groups; i0 += 32) {
         const int i = i0 + lane;
         const bool in = i < 2 * p.n_groups;
-        const int64_t unit = (int64_t) (i >> 1) * p.n_row_tiles + row_tile;
-        const int64_t slot = (unit * cg + rank) * 2 + (i & 1);
+        const int64_t slot = part_slot(p, cg, row, i);
         unsigned long long k = in && p.n_top ? p.part_keys[slot * p.n_top * 128 + place] : 0ull;
         if (in) {
             const float4 s = p.part_stats[slot * 128 + place];
@@ -442,26 +441,88 @@ __global__ void __launch_bounds__(kJoinWarps * 32) head_join_kernel(const HeadSc
         }
         for (int j = 0; j < p.n_top; ++j) {
             if (j) k = in ? p.part_keys[(slot * p.n_top + j) * 128 + place] : 0ull;
-            if (j == 0 && top.low == 0ull) top.bound((uint32_t) (k >> 32));
+            if (j == 0 && i0 == 0) top.bound((uint32_t) (k >> 32));
             if (!__any_sync(kAll, k > top.low)) break;  // the parts' lists are in order
             top.offer(k);
         }
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) a = stat_join(a, stat_shfl_xor(a, o));
-    if constexpr (WARPS > 1) {
-        if (lane == 0) stats[warp] = a;
-        if (lane < p.n_top) lists[warp * p.n_top + lane] = top.key;
-        __syncthreads();
-        if (warp != 0) return;
-        a = lane < kJoinWarps ? stats[lane] : stat_empty();
-#pragma unroll
-        for (int o = kJoinWarps / 2; o >= 1; o >>= 1) a = stat_join(a, stat_shfl_xor(a, o));
-        a = {__shfl_sync(kAll, a.m, 0), __shfl_sync(kAll, a.s, 0), __shfl_sync(kAll, a.t, 0)};
-        for (int i = p.n_top; i < kJoinWarps * p.n_top; i += 32)  // the warp's own list is in place
-            top.offer(i + lane < kJoinWarps * p.n_top ? lists[i + lane] : 0ull);
-    }
     score_write(out, row, a, top.key, token, token_logit);
+}
+
+// The same by a CTA, a thread one part: few rows, of many parts.  The keys that reach the
+// row's bound are ranked against each other.
+constexpr int kJoinKeys = 2 * kMostGroups * kMaxTop;
+__global__ void __launch_bounds__(kJoinWarps * 32) head_join_block_kernel(const HeadScoreParams p, const ScoreOut out, int cg) {
+    __shared__ Stat stats[kJoinWarps];
+    __shared__ unsigned long long keys[kJoinKeys], best[kMaxTop], group[64], bound;
+    __shared__ int count;
+    constexpr int kThreadsOfRow = kJoinWarps * 32;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = (int) blockIdx.x, place = row % 128;
+    const int n_top = p.n_top, n_parts = 2 * p.n_groups;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int32_t token = out.tokens ? out.tokens[row] : -1;
+    const float token_logit = p.token_logits[row];
+    const uint32_t low = n_top ? p.row_low[row] : 0u;
+    Stat a = stat_empty();
+    unsigned long long first[2] = {0ull, 0ull};  // its parts' largest keys
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int i = tid + t * kThreadsOfRow;
+        if (i < n_parts) {
+            const int64_t slot = part_slot(p, cg, row, i);
+            const float4 s = p.part_stats[slot * 128 + place];
+            if (n_top) first[t] = p.part_keys[slot * n_top * 128 + place];
+            a = stat_join(a, Stat{s.x, s.y, s.z});
+        }
+    }
+    if (tid == 0) {
+        count = 0;
+        bound = (unsigned long long) low << 32;
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) a = stat_join(a, stat_shfl_xor(a, o));
+    if (lane == 0) stats[warp] = a;
+    if (n_top) {  // the n_top-th largest of 64 groups' keys bounds the list closer than any one part could
+        unsigned long long g = max(first[0], first[1]);
+        g = max(g, __shfl_xor_sync(kAll, g, 1));
+        g = max(g, __shfl_xor_sync(kAll, g, 2));
+        if (tid % 4 == 0) group[tid / 4] = g;
+        __syncthreads();
+        if (tid < 64) {
+            int above = 0;
+            for (int j = 0; j < 64; ++j) above += group[j] > group[tid];
+            if (above == n_top - 1 && group[tid] > bound) bound = group[tid];  // keys differ: one thread
+        }
+    }
+    __syncthreads();
+    const unsigned long long least = bound;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int64_t slot = part_slot(p, cg, row, tid + t * kThreadsOfRow);
+        unsigned long long k = first[t];
+        for (int j = 0; k && k >= least; ) {
+            keys[atomicAdd(&count, 1)] = k;
+            if (++j == n_top) break;
+            k = p.part_keys[(slot * n_top + j) * 128 + place];  // a part's list is in order
+        }
+    }
+    __syncthreads();
+    const int n = count;
+    for (int i = tid; i < n; i += kThreadsOfRow) {
+        const unsigned long long mine = keys[i];
+        int above = 0;
+        for (int j = 0; j < n; ++j) above += keys[j] > mine;
+        if (above < n_top) best[above] = mine;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    a = lane < kJoinWarps ? stats[lane] : stat_empty();
+#pragma unroll
+    for (int o = kJoinWarps / 2; o >= 1; o >>= 1) a = stat_join(a, stat_shfl_xor(a, o));
+    a = {__shfl_sync(kAll, a.m, 0), __shfl_sync(kAll, a.s, 0), __shfl_sync(kAll, a.t, 0)};
+    score_write(out, row, a, lane < min(n, n_top) ? best[lane] : 0ull, token, token_logit);
 }
 
 template <int DT, int CG, int LIST>
@@ -507,7 +568,7 @@ HeadScorePlan head_score_plan(int32_t n_rows, int32_t vocab, int sms) {
     HeadScorePlan c{};
     c.cg = n_rows <= 128 ? 1 : 2;
     c.n_row_tiles = (n_rows + 128 * c.cg - 1) / (128 * c.cg);
-    const int64_t groups = std::max(1, sms / c.cg / c.n_row_tiles);
+    const int64_t groups = std::min(kMostGroups, std::max(1, sms / c.cg / c.n_row_tiles));
     const int64_t rounds = (vocab + groups * 256 - 1) / (groups * 256);
     const int64_t cols = ((int64_t) vocab + groups * rounds - 1) / (groups * rounds);
     c.tile_cols = (int32_t) std::min<int64_t>(256, (cols + 31) / 32 * 32);
@@ -536,6 +597,7 @@ cudaError_t launch_head_score(const HeadScoreParams & p, const ScoreOut & out, c
     }
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
+    // a warp takes 64 parts in two turns; with more the CTA's barriers are the shorter way
     const bool many = 2 * p.n_groups > 64;
     cfg.gridDim = dim3((unsigned) (many ? p.n_rows : (p.n_rows + kJoinWarps - 1) / kJoinWarps));
     cfg.blockDim = dim3(kJoinWarps * 32);
@@ -545,8 +607,8 @@ cudaError_t launch_head_score(const HeadScoreParams & p, const ScoreOut & out, c
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return many ? cudaLaunchKernelEx(&cfg, head_join_kernel<kJoinWarps>, p, out, cg)
-                : cudaLaunchKernelEx(&cfg, head_join_kernel<1>, p, out, cg);
+    return many ? cudaLaunchKernelEx(&cfg, head_join_block_kernel, p, out, cg)
+                : cudaLaunchKernelEx(&cfg, head_join_warp_kernel, p, out, cg);
 }
 
 }  // namespace vxk
