@@ -98,6 +98,7 @@ def test_score_call_refusals(vxk):
     refused(head.score, 0, a, 1, a, 0, a, a, a, a)
     refused(head.score, a, 0, 1, a, 0, a, a, a, a)
     refused(head.score, a + 8, a, 1, a, 0, a, a, a, a)
+    refused(head.score, a, a + 4, 1, a, 0, a, a, a, a)
     refused(head.score, a, a, 1, a, 17, a, a, a, a)
     head.close()
 

@@ -145,7 +145,8 @@ void need_score_scratch(vxk_head * h, cudaStream_t cs) {
     if (st != cudaStreamCaptureStatusNone)
         hfail(VXK_STATUS_INVALID_STATE, "the first scoring call of a head allocates: make it outside a stream capture");
     const size_t ctas = (size_t) h->sm_count * vxk::kScoreCtasPerSm;
-    const size_t slots = (size_t) h->sm_count * 2 * 128;  // rows of all epilogue halves
+    // rows of all epilogue halves; a row tile has a CTA however few multiprocessors there are
+    const size_t slots = (size_t) std::max(h->sm_count, vxk::kScoreRows / 128) * 2 * 128;
     size_t at = 0;
     auto take = [&at](size_t bytes) {
         const size_t here = at;
@@ -354,7 +355,8 @@ vxk_status vxk_head_score(vxk_head * head, const void * w, const float * x, int3
     return hguarded(head, [&] {
         const vxk_head_config & c = head->cfg;
         if (!w || !x) hfail(VXK_STATUS_INVALID_ARGUMENT, "null buffer");
-        if (reinterpret_cast<uintptr_t>(w) % 16 != 0) hfail(VXK_STATUS_INVALID_ARGUMENT, "w must be 16-byte aligned");
+        if ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(x)) % 16 != 0)
+            hfail(VXK_STATUS_INVALID_ARGUMENT, "w and x must be 16-byte aligned");
         const vxk::ScoreOut out = score_out(head, rows, tokens, n_top, logprob, entropy, top_ids, top_logprobs);
         HeadDevice scope(c.device);
         cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
