@@ -521,8 +521,8 @@ VXK_API vxk_status vxk_head_score_logits(vxk_head * head, const void * logits, v
  * products, the softmax statistics and the top lists are one kernel, and W is
  * read once per 2048 rows.  x is rounded to W's type as in
  * vxk_head_logits_argmax; the tensor cores' sums are moved to fp32 registers
- * every 256 columns.
- *   w  [vocab][dim] f16 or bf16, device, 16-byte aligned;  x [rows][dim] fp32
+ * every 256 columns (f16) or 512 (bf16).
+ *   w  [vocab][dim] f16 or bf16;  x [rows][dim] fp32;  device, 16-byte aligned
  * Everything else as in vxk_head_score_logits.
  */
 VXK_API vxk_status vxk_head_score(vxk_head * head, const void * w, const float * x, int32_t rows,
@@ -577,7 +577,8 @@ VXK_API vxk_status vxk_prompt_last_error(const vxk_prompt * prompt, char * buf, 
  * behind the calls still using the old one.  Refused inside a stream capture.
  * Calls captured into a graph use, at each replay, the plan of that time; a
  * plan with more rows than the one they were captured under makes them write
- * nothing and report a device error.
+ * nothing and report a device error (under a plan without rows nothing is
+ * launched, so nothing is captured).
  */
 VXK_API vxk_status vxk_prompt_plan(vxk_prompt * prompt, const int32_t * n_rows, const int32_t * first_position,
                                    int32_t n_seqs, void * cuda_stream);
@@ -815,10 +816,11 @@ VXK_API vxk_status vxk_decoder_forward(vxk_decoder * d, const int32_t * tokens, 
  * token gives the log probability of given[r], its entropy and its n_top most
  * likely tokens (vxk_head_score; the outputs are its, per row).  With a
  * transcript's tokens and given[r] = tokens[r + 1] these are the transcript's
- * word confidences.  Streams that begin with the batch are attended as packed
- * prompts (vxk_prompt_attention, 16-bit rows), others over the cache
- * (vxk_attend_layer); either way the caches are appended as in
- * vxk_decoder_forward and the caller commits, or aborts to leave no trace.
+ * word confidences.  A batch of 64 rows or more whose streams all begin with
+ * it is attended as packed prompts (vxk_prompt_attention, f16 rows), any other
+ * one, or one of an F32 cache, over the cache (vxk_attend_layer); the caches
+ * are appended as in vxk_decoder_forward and the caller commits, or aborts to
+ * leave no trace.
  *   given  [rows] host array, < vocab; a negative one is not scored
  * Asynchronous on cuda_stream; the first call allocates its scratch.
  */

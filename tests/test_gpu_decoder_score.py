@@ -150,6 +150,40 @@ def test_streams_with_a_past_are_scored_over_the_cache(vxk, tmp_path):
         pool.close()
 
 
+@pytest.mark.parametrize("cache,past", [(0, 0), (1, 5)], ids=["f32 cache", "one stream with a past"])
+def test_prompts_that_are_not_packed(vxk, tmp_path, cache, past):
+    """Whole prompts of an F32 cache, and ones beside a stream with a past, are attended over the
+    cache: the forward's own log probabilities."""
+    import torch
+
+    _, pool, dec = _setup(vxk, tmp_path, 71 + past, cache=cache)
+    rng = np.random.default_rng(10)
+    vocab = dec.info["vocab"]
+    streams, lens = [pool.open_stream(), pool.open_stream()], [60, 11]
+    amax = torch.zeros(2, dtype=torch.int32, device="cuda")
+    if past:
+        pool.plan(streams[1:], [past], _stream())
+        dec.forward([3] * past, [0] * past, amax.data_ptr(), cuda_stream=_stream())
+        dec.sync(_stream())
+        pool.commit()
+    tokens = [int(t) for t in rng.integers(0, vocab, 71)]
+    given = [int(t) for t in rng.integers(0, vocab, 71)]
+    pool.plan(streams, lens, _stream())
+    lp, _, _, _ = _score(dec, tokens, [0] * 71, given, 0)
+    pool.abort()
+    pool.plan(streams, lens, _stream())
+    logits = torch.empty(2, vocab, device="cuda")
+    dec.forward(tokens, [0] * 71, amax.data_ptr(), logits.data_ptr(), cuda_stream=_stream())
+    dec.sync(_stream())
+    pool.commit()
+    l = logits.cpu().numpy().astype(np.float64)
+    want = _log_softmax(l)
+    for s, r in enumerate((59, 70)):
+        assert abs(lp[r] - want[s, given[r]]) <= EXACT_BAR * np.abs(l).max()
+    dec.close()
+    pool.close()
+
+
 def test_decoding_goes_on_behind_a_scored_prompt(vxk, tmp_path):
     """The caches of a scored prompt are those of a prefill: the first layer's bytes, and the next token's logits."""
     import torch

@@ -584,6 +584,9 @@ struct ScoreCall {
     float * top_logprobs;
 };
 
+// Fewest rows of a batch worth the packed attention's three launches.
+constexpr int32_t kPackedRows = 64;
+
 // The scoring state of a decoder, allocated once.
 void need_score(vxk_decoder * d) {
     if (d->prompt) return;
@@ -649,8 +652,11 @@ void forward(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slot
             if (sc->given[r] >= d->vocab) dfail(VXK_STATUS_INVALID_ARGUMENT, "given token out of range");
         need_score(d);
         upload(d, sc->given, (size_t) rows * sizeof(int32_t), d->d_given, cs);
-        // Streams that begin with this batch attend its rows alone.
-        packed = !bv.single_token;
+        // Streams that begin with this batch attend its rows alone; an f32 cache asks for
+        // more than 16-bit rows.  A layer's attention over the cache (32 / 8 heads of 128)
+        // against the packed one, of which 2-3 us are the widened rows: 2 rows 6 / 15 us,
+        // 38 rows 16 / 17, 8 x 38 rows 41 / 17, 512 rows 105 / 25, 4000 rows 3050 / 155.
+        packed = rows >= kPackedRows && !bv.single_token && d->ps.dtype != VXK_DTYPE_F32;
         std::vector<int32_t> lens;
         for (int32_t i = 0, r0 = 0; i < n_out; r0 = bv.last_rows[(size_t) i] + 1, ++i) {
             lens.push_back(bv.last_rows[(size_t) i] + 1 - r0);

@@ -527,6 +527,7 @@ bool pool_batch_view(const vxk_pool * pool, PoolBatchView * out);
 struct PoolShape {
     int32_t device, n_layers, n_q, n_kv, head_dim, max_streams, max_rows;
     float rope_theta;
+    int32_t dtype;  // vxk_dtype of the pages
 };
 PoolShape pool_shape(const vxk_pool * pool);
 // The pool's RoPE table, [rows][head_dim / 2] (cos, sin) on its device.

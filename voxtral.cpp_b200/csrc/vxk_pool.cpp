@@ -636,7 +636,7 @@ bool pool_batch_view(const vxk_pool * pool, PoolBatchView * out) {
 PoolShape pool_shape(const vxk_pool * pool) {
     const vxk_pool_config & c = pool->cfg;
     return PoolShape{c.device, c.n_layers, c.n_q_heads, c.n_kv_heads, c.head_dim, c.max_streams, c.max_rows,
-                     c.rope_theta};
+                     c.rope_theta, (int32_t) c.dtype};
 }
 
 const float2 * pool_rope_table(const vxk_pool * pool, int32_t * rows) {
