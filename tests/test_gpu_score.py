@@ -95,7 +95,8 @@ def check(got, l64, tokens, n_top):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("rows,vocab,pad,n_top", [
     (1, 1, 0, 1), (3, 7, 1, 5), (2, 33, 0, 16), (19, 511, 3, 1), (5, 4096, 0, 8), (9, 4097, 5, 16), (1, 131072, 0, 16),
-    (3, 131071, 0, 4), (301, 12289, 2, 3), (700, 40, 7, 2), (64, 32003, 0, 0), (2, 300007, 1, 16)])
+    (3, 131071, 0, 4), (301, 12289, 2, 3), (700, 40, 7, 2), (64, 32003, 0, 0), (2, 300007, 1, 16),
+    (500, 32003, 1, 5), (460, 70000, 0, 2)])
 def test_logits_match_the_definition(vxk, dtype, rows, vocab, pad, n_top):
     import torch
 

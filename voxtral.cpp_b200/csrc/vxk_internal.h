@@ -278,6 +278,7 @@ struct ScoreLogitsParams {
     int64_t ld;
     int64_t rows;
     int64_t strips;        // strips of a row (set by the launch)
+    int64_t unit;          // strips that stay with one CTA: 1, or a row's (set by the launch)
     int32_t dtype;         // 0 = f32, 1 = f16, 30 = bf16
     ScorePart * parts;     // [2 x kScoreCtasPerSm x SMs]
     int32_t * counters;    // [kScoreCtasPerSm x SMs], zero between launches
