@@ -231,7 +231,8 @@ def test_same_results_every_time_and_inside_a_graph(vxk):
 # values are exact in fp32; a step adds 16 of them to the running sum, dropping bits
 # below 2^-23 = 2 U of it, for 16 steps a 256-column piece in f16 and 32 steps a
 # 512-column piece in bf16; the pieces are added in fp32, U each, dim / 256 of them at
-# most), so at most (32 + dim / 256 + 2) 2 U A with A = sum |x_i w_i| of the logit, and
+# most; giving back the mean of what is dropped adds no more than was dropped at most),
+# so at most (32 + dim / 256 + 2) 2 U A with A = sum |x_i w_i| of the logit, and
 # none for x's rounding to W's type, which belongs to the definition.  A logit off by D
 # moves a log probability by 2 D at most (its own and log s), the entropy by
 # 2 D (1 + H + log s...) <= 2 D (2 + the largest |log p| that matters).

@@ -18,7 +18,10 @@
 // every step: over 4096 columns the largest logits come out 6e-6 too small, and the
 // entropy 4e-5 off.  So a sum is taken out every 512 columns (bf16) or 256 (f16, whose
 // products have six bits more to lose), two accumulators in turn in TMEM, and added up
-// in fp32 registers: 128 columns a thread, eight epilogue warps.
+// in fp32 registers: 128 columns a thread, eight epilogue warps.  What is dropped in
+// the mean (dropped_share) is given back, one FMA a logit: entropies of 700 rows of
+// 2048 columns are then 1.1e-6 off (bf16) or 2.5e-6 (f16) instead of 4.3e-6 and 4.9e-6;
+// a plain fp32 product's are 5e-6 off.
 //
 // A row's top list is found by 2 n_groups threads, each over its own columns.  What
 // one thread knows of the list's end bounds it for all, so they share the largest such
@@ -65,9 +68,22 @@ struct Shape {
     static constexpr int kBars = kDrain + 1;
 };
 
-// Chunks summed in TMEM before they are moved to registers.
+// Chunks summed in TMEM before they are moved to registers; 2 for up to kFewRows rows of
+// f16, where that halves the error again and costs 0-1 % (32 rows: 6 %).
 template <int DT>
 constexpr int kSegmentOf = DT == 30 ? 8 : 4;
+constexpr int kFewRows = 16;
+
+// What the accumulation drops of a sum on average, relative to it.  A step (16 columns)
+// truncates the running sum at 2^-23 of its power of two: half a unit of it is lost in the
+// mean, 2^-24 E[2^floor(log2 x) / x] = 2^-24 / (2 ln 2) of the running sum x, which over
+// the steps of a segment averages half of the segment's.
+__device__ __forceinline__ float dropped_share(int n_chunks, int segment) {
+    constexpr float kStep = 0.72134752f / (1 << 25);
+    const int whole = n_chunks / segment, rest = n_chunks % segment;
+    // segments weigh in by their columns
+    return kStep * 4.0f * (float) (whole * segment * segment + rest * rest) / (float) n_chunks;
+}
 
 // One thread's list of its largest keys, largest first.  LIST 0: none; up to 4 places in
 // registers (an insertion is four compares and swaps); up to 16 in shared memory, the
@@ -135,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                                                                  const __grid_constant__ CUtensorMap tmx,
                                                                  const HeadScoreParams p) {
     using S = Shape<CG>;
-    constexpr int kSegment = kSegmentOf<DT>;
+    const int segment = DT == 1 && p.n_rows <= kFewRows ? 2 : kSegmentOf<DT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t * base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned long long * lists = reinterpret_cast<unsigned long long *>(base + kRing);
@@ -149,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
     const int row_tile = unit % p.n_row_tiles, group = unit / p.n_row_tiles;
     const int row0 = row_tile * (128 * CG) + rank * 128;  // this CTA's first row
     const int n_chunks = p.dim / kChunk;
-    const int n_segs = (n_chunks + kSegment - 1) / kSegment;
+    const int n_segs = (n_chunks + segment - 1) / segment;
 
     if (tid == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -222,8 +238,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t d = tmem + 256 * b;
-                    const int last = min(n_chunks, (s + 1) * kSegment);
-                    for (int ch = s * kSegment; ch < last; ++ch) {
+                    const int last = min(n_chunks, (s + 1) * segment);
+                    for (int ch = s * segment; ch < last; ++ch) {
                         ok = uniform(tc_wait(&bars[S::kFull + st], par, abort_flag, p.error));
                         if (!ok) break;
                         tc_fence_after();
@@ -232,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                         if (elect_one()) {
 #pragma unroll
                             for (int ks = 0; ks < 4; ++ks)  // 32 bytes further: 2 in the descriptor's 16-byte units
-                                tc_mma<CG>(d, da + 2 * ks, db + 2 * ks, idesc, (ch != s * kSegment) | (ks != 0));
+                                tc_mma<CG>(d, da + 2 * ks, db + 2 * ks, idesc, (ch != s * segment) | (ks != 0));
                             tc_commit<CG>(&bars[S::kEmpty + st]);
                             if (ch + 1 == last) tc_commit<CG>(&bars[S::kDFull + b]);
                         }
@@ -265,9 +281,11 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
         const bool listed = LIST != 0 && row < p.n_rows;
         asm volatile("griddepcontrol.wait;" ::: "memory");
         const int32_t token = p.tokens && row < p.n_rows ? p.tokens[row] : -1;
+        const float dropped = dropped_share(n_chunks, segment);
         Stat a = stat_empty();
         uint32_t seg = 0;  // two accumulators in turn: bit 0, and the parity in bit 1
         bool have = true;
+        const bool rows_here = row0 + q * 32 < p.n_rows;  // the same for a warp
         for (int tile = group; have && tile < p.n_tiles; tile += p.n_groups) {
             float acc[kHalfCols];
             for (int s = 0; s < n_segs; ++s, ++seg) {
@@ -277,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                 tc_fence_after();
 #pragma unroll
                 for (int c0 = 0; c0 < kHalfCols; c0 += 32) {
+                    if (!rows_here) break;
                     float v[32];
                     tmem_ld32(tmem + 256 * b + lane_off + c0, v);
 #pragma unroll
@@ -287,8 +306,11 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                 if (lane == 0) mbar_arrive_cluster<CG>(&bars[S::kDEmpty + b], 0);
             }
             if (!have) break;
+            if (!rows_here) continue;
             // the row's bound so far, on its way while the statistics are taken
             uint32_t bound = listed && tile != group ? __ldcg(&p.row_low[row]) : 0u;
+#pragma unroll
+            for (int j = 0; j < kHalfCols; ++j) acc[j] = fmaf(acc[j], dropped, acc[j]);
             const int col0 = tile * p.tile_cols + half * n_half;
             const int limit = min(n_half, p.vocab - col0);
             if (limit < kHalfCols) {
