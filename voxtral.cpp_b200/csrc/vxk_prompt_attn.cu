@@ -244,25 +244,6 @@ __device__ __forceinline__ void scale_o(uint32_t to, float f) {
     }
 }
 
-// A step of turning the 4 x 4 matrix whose rows are four neighbouring lanes' h, each in four
-// eights: lanes DIST apart swap the eights that are DIST apart.  After the steps of 2 and of 1
-// a lane holds the eight of its own place out of each of the four rows.
-template <int DIST>
-__device__ __forceinline__ void quad_transpose(uint32_t (&h)[32], int lane) {
-    const bool upper = lane & DIST;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (j & DIST) continue;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            uint32_t &a = h[8 * j + e], &b = h[8 * (j + DIST) + e];
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? a : b, DIST);
-            if (upper) a = got;
-            else b = got;
-        }
-    }
-}
-
 // One thread's running state over the keys of its row.
 struct RowState {
     float m;             // what p is taken from, in score units
@@ -609,19 +590,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             if (!ok) break;
             tc_fence_after();
             const bool bad = v_flags[(i - begin) % kFlags] | v_flags[kFlags + (i - begin) % kFlags];
+            const int head = it.head + (r & ((1 << p.pack_shift) - 1));
             const float f = 1.0f / row.sum;
+            uint16_t * out = static_cast<uint16_t *>(p.out) + ((int64_t) (it.row0 + token) * p.n_q + head) * HD;
 #pragma unroll
-            for (int k = 0; k < HD; k += 64) {
-                uint32_t h[32];  // 64 dims of the row: a 128-byte line
-#pragma unroll
-                for (int k2 = 0; k2 < 64; k2 += 32) {
-                    uint32_t o[32];
-                    tmem_load32(to + k + k2, o);
-                    tmem_wait_ld();
+            for (int k = 0; k < HD; k += 32) {
+                uint32_t o[32];
+                tmem_load32(to + k, o);
+                tmem_wait_ld();
+                if (token < it.len) {
                     float y[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * f;
-                    if (bad && token < it.len) {
+                    if (bad) {
                         for (int t = 0; t < it.tiles(); ++t) {
                             if (!it.masked(t, p)) continue;
                             const int k0 = (it.lo + t) * kTile;
@@ -629,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                             const int upto = min(k0 + kTile, p.causal ? token + 1 : it.len);
                             for (int key = from; key < upto; ++key) {
                                 const uint16_t * v = static_cast<const uint16_t *>(p.v) +
-                                                     ((int64_t) (it.row0 + key) * p.n_kv + it.head / p.group) * HD + k + k2;
+                                                     ((int64_t) (it.row0 + key) * p.n_kv + it.head / p.group) * HD + k;
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) {
                                     const uint16_t w = v[e];
@@ -638,26 +619,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                             }
                         }
                     }
+                    uint32_t h[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) h[k2 / 2 + e] = cvt2<DT>(y[2 * e], y[2 * e + 1]);
-                }
-                // Four lanes turn their four rows' lines, so that a store of theirs is one line:
-                // a quarter of the requests, 1.3 % of a long sequence's time.
-                quad_transpose<2>(h, lane);
-                quad_transpose<1>(h, lane);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int rj = (r & ~3) + j, tj = first + (rj >> p.pack_shift);
-                    if (tj >= it.len) continue;
-                    const int head = it.head + (rj & ((1 << p.pack_shift) - 1));
-                    uint16_t * out = static_cast<uint16_t *>(p.out) + ((int64_t) (it.row0 + tj) * p.n_q + head) * HD + k +
-                                     16 * (lane & 3);
-                    if (p.out_32) {
-                        store_32(out, h + 8 * j);
+                    for (int e = 0; e < 16; ++e) h[e] = cvt2<DT>(y[2 * e], y[2 * e + 1]);
+                    if (p.out_32) {  // whole sectors: half the requests
+                        store_32(out + k, h);
+                        store_32(out + k + 16, h + 8);
                     } else {
-                        *reinterpret_cast<uint4 *>(out) = make_uint4(h[8 * j], h[8 * j + 1], h[8 * j + 2], h[8 * j + 3]);
-                        *reinterpret_cast<uint4 *>(out + 8) =
-                            make_uint4(h[8 * j + 4], h[8 * j + 5], h[8 * j + 6], h[8 * j + 7]);
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            *reinterpret_cast<uint4 *>(out + k + 2 * e) = make_uint4(h[e], h[e + 1], h[e + 2], h[e + 3]);
                     }
                 }
             }
