@@ -23,6 +23,12 @@
 // 2048 columns are then 1.1e-6 off (bf16) or 2.5e-6 (f16) instead of 4.3e-6 and 4.9e-6;
 // a plain fp32 product's are 5e-6 off.
 //
+// Measured (bf16): 100 rows x 131072 x 2048 102 us with lists of 4, 5.3 TB/s of W (93 without:
+// 5.8); 2000 rows x 131072 x 4096 1590 us, 1.35 PFLOP/s (without lists 1450, 1.48; a plain
+// library product reaches 1.66 in a burst and 1.39 under the power cap); 5 rows of f16 x
+// 32000 x 1280 29 us, of which three launches and the join are 14.  The lists' cost
+// is the few candidates behind each row's bound, looked for by every thread of a tile.
+//
 // A row's top list is found by 2 n_groups threads, each over its own columns.  What
 // one thread knows of the list's end bounds it for all, so they share the largest such
 // bound in global memory (row_low) and few candidates are left to any of them; the

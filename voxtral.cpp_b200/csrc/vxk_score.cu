@@ -14,6 +14,11 @@
 // takes 16 elements of each and their maximum first, so that the sums are rescaled at
 // most once a strip.
 //
+// Measured: 600 rows of 131072 f32 logits 58 us without a list (5.4 TB/s, 83 % of a copy's
+// rate; two CTAs or deeper rings were no faster) and 72 with one of 8; 333 rows of 32003
+// bf16 15 and 18 us; four rows 12 us, one launch, in which a row's parts are written,
+// counted in and joined behind one strip a CTA.
+//
 // The top list costs the scan nothing but each thread's running maximum, noted a dozen
 // times a run.  Behind the run the n_top-th largest of 64 groups' maxima bounds the
 // list's end from below; the few noted maxima that reach it name the elements to read
