@@ -121,6 +121,15 @@ def test_whole(vxk, dim, heads, kv):
         check_attention(attend(vxk, q, k, v, lens, BF16, causal=0), q, k, v, lens, BF16, causal=0)
 
 
+@pytest.mark.parametrize("dim,heads,kv,lens,causal,window", [
+    (64, 20, 20, [600] * 5 + [300, 129], 0, 0), (128, 32, 8, [200] * 13 + [1] * 9, 1, 0), (64, 12, 12, [500] * 7, 1, 140)])
+def test_more_items_than_ctas(vxk, dim, heads, kv, lens, causal, window):
+    """Several items a CTA, of every number of key tiles."""
+    q, k, v = make(lens, heads, kv, dim, F16)
+    out = attend(vxk, q, k, v, lens, F16, causal=causal, window=window)
+    check_attention(out, q, k, v, lens, F16, causal=causal, window=window)
+
+
 @pytest.mark.parametrize("window", [1, 2, 63, 64, 128, 129, 300, 10000])
 def test_window(vxk, window):
     lens = [500, 1, 129, 64]
