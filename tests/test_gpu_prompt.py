@@ -261,6 +261,40 @@ def test_another_stream_and_an_empty_plan(vxk):
     prompt.close()
 
 
+def test_offsets_beyond_32_bits(vxk):
+    """530,000 rows of 32 heads of 128: more than 2^31 values of q and of the output."""
+    import torch
+
+    lens, heads, dim, dtype = [1000] * 529 + [937, 63], 32, 128, F16
+    rows, tail = sum(lens), 1000
+    g = torch.Generator(device="cuda").manual_seed(11)
+    prompt = vxk.Prompt(n_q_heads=heads, n_kv_heads=1, head_dim=dim, max_seqs=len(lens), max_rows=rows, max_position=1000,
+                        dtype=dtype)
+    prompt.plan(lens, cuda_stream=_stream())
+    q = torch.zeros(rows, heads, dim, device="cuda")
+    k, v = torch.zeros(rows, 1, dim, device="cuda"), torch.zeros(rows, 1, dim, device="cuda")
+    for x in (q, k, v):
+        x[-tail:] = torch.randn(x[-tail:].shape, generator=g, device="cuda")
+    q16, k16, v16 = (torch.full(x.shape, 9.0, dtype=torch.float16, device="cuda") for x in (q, k, v))
+    prompt.rope(*(x.data_ptr() for x in (q, k, v, q16, k16, v16)), _stream())
+    prompt.sync(_stream())
+    small = vxk.Prompt(n_q_heads=heads, n_kv_heads=1, head_dim=dim, max_seqs=2, max_rows=tail, max_position=1000, dtype=dtype)
+    small.plan([937, 63], cuda_stream=_stream())
+    want = [torch.empty_like(x[-tail:]) for x in (q16, k16, v16)]
+    small.rope(*(x[-tail:].contiguous().data_ptr() for x in (q, k, v)), *(x.data_ptr() for x in want), _stream())
+    small.sync(_stream())
+    for x, y in zip((q16, k16, v16), want):
+        assert torch.equal(x[-tail:], y) and bool((x[: tail] == 0).all())
+    del q
+    out = torch.full_like(q16, 9.0)
+    prompt.attention(q16.data_ptr(), k16.data_ptr(), v16.data_ptr(), out.data_ptr(), _stream())
+    prompt.sync(_stream())
+    check_attention(out[-tail:], q16[-tail:], k16[-tail:], v16[-tail:], [937, 63], dtype)
+    assert bool((out[: -tail] == 0).all())
+    prompt.close()
+    small.close()
+
+
 # ---- rotary rows --------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [F16, BF16])

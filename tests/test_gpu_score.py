@@ -108,6 +108,22 @@ def test_logits_match_the_definition(vxk, dtype, rows, vocab, pad, n_top):
     check(score_logits(vxk, l, vocab, tokens, n_top), l[:, :vocab].double().cpu().numpy(), tokens, n_top)
 
 
+def test_offsets_beyond_32_bits(vxk):
+    """17,000 rows of 131,072 logits: more than 2^31; all but a few rows are even."""
+    import torch
+
+    rows, vocab = 17000, 131072
+    l = torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    torch.manual_seed(9)
+    some = [0, 8191, 16383, 16384, 16999]
+    l[some] = torch.randn(len(some), vocab, device="cuda").bfloat16() * 3
+    got = score_logits(vxk, l, vocab, np.full(rows, 77), 3)
+    check([x[some] for x in got], l[some].double().cpu().numpy(), np.full(len(some), 77), 3)
+    even = np.setdiff1d(np.arange(rows), some)
+    assert np.allclose(got[0][even], -np.log(vocab), rtol=1e-5) and np.allclose(got[1][even], np.log(vocab), rtol=1e-5)
+    assert np.array_equal(got[2][even], np.tile([0, 1, 2], (len(even), 1)))
+
+
 def test_equal_logits_list_the_lowest_index_first(vxk):
     import torch
 
