@@ -74,8 +74,10 @@ struct Shape {
     static constexpr int kBars = kDrain + 1;
 };
 
-// Chunks summed in TMEM before they are moved to registers; 2 for up to kFewRows rows of
-// f16, where that halves the error again and costs 0-1 % (32 rows: 6 %).
+// Chunks summed in TMEM before they are moved to registers; 2 for up to kFewRows rows,
+// where that brings f16's error down to half and bf16's to two thirds and costs 0-3 %
+// (32 rows of f16: 6 %).  One chunk at a time is no more exact: the fp32 adds are then what
+// is left, a unit or two in a logit's last place.
 template <int DT>
 constexpr int kSegmentOf = DT == 30 ? 8 : 4;
 constexpr int kFewRows = 16;
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                                                                  const __grid_constant__ CUtensorMap tmx,
                                                                  const HeadScoreParams p) {
     using S = Shape<CG>;
-    const int segment = DT == 1 && p.n_rows <= kFewRows ? 2 : kSegmentOf<DT>;
+    const int segment = p.n_rows <= kFewRows ? 2 : kSegmentOf<DT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t * base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned long long * lists = reinterpret_cast<unsigned long long *>(base + kRing);
