@@ -1,0 +1,63 @@
+"""Scores of logits and of hidden rows at the edges of their definition, through the C ABI."""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = 0, 1, 30
+
+
+def _stream():
+    import torch
+
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _torch_type(dtype):
+    import torch
+
+    return {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}[dtype]
+
+
+def _outputs(rows, n_top):
+    import torch
+
+    return (torch.full((rows,), 7.0, device="cuda"), torch.full((rows,), 7.0, device="cuda"),
+            torch.full((rows, n_top), -7, dtype=torch.int32, device="cuda"), torch.full((rows, n_top), 7.0, device="cuda"))
+
+
+def _score_logits(vxk, l, dtype, vocab, tokens, n_top):
+    import torch
+
+    head = vxk.Head(dim=64, vocab=vocab)
+    outs = _outputs(len(l), n_top)
+    tok = torch.as_tensor(tokens, dtype=torch.int32, device="cuda")
+    head.score_logits(l.data_ptr(), dtype, l.stride(0), len(l), tok.data_ptr(), n_top, *(o.data_ptr() for o in outs), _stream())
+    head.sync(_stream())
+    head.close()
+    return outs
+
+
+def _lowest_first(l, n_top):
+    import torch
+
+    return torch.sort(l.float(), dim=1, descending=True, stable=True)[1][:, :n_top].int()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n_top", [1, 2, 3, 16])
+@pytest.mark.parametrize("rows,vocab", [(500, 70001), (460, 70003), (160, 133333)])
+def test_ties_with_the_ragged_end_of_a_row(vxk, dtype, n_top, rows, vocab):
+    """Runs of many strips, the first of them lower, all behind it equal up to the row's last element."""
+    import torch
+
+    l = torch.zeros(rows, vocab, device="cuda")
+    l[:, :4096] = -1.0
+    l[1::4, : 3 * 4096 + 5] = -1.0
+    l[2::4, 20000:] = 1.0
+    l[3::4] = torch.randint(0, 3, l[3::4].shape, device="cuda").float()
+    l = l.to(_torch_type(dtype))
+    ids = _score_logits(vxk, l, dtype, vocab, torch.zeros(rows), n_top)[2]
+    assert torch.equal(ids, _lowest_first(l, n_top))
+    assert ids[0, 0] == 4096 and ids[1, 0] == 3 * 4096 + 5 and ids[2, 0] == 20000

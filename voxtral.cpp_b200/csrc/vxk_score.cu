@@ -315,11 +315,15 @@ __device__ __forceinline__ void select(Collected & c, const Row<DT> & r, int c0,
         const int v0 = s * kStep + tid;
         float x[E::kPer];
         take_strip<DT, false>(r, r.body + (int64_t) v0 * 16, v0, kThreads, x);
-        // A later element of the list's last value stands behind it.
-        const uint32_t last = (uint32_t) (c.bound >> 32);
+        // Whole keys: the list's last may be one of the row's last elements, which are in it from
+        // the start, and an element of the same value here stands before it.
+        const unsigned long long last = c.bound;
         bool any = false;
 #pragma unroll
-        for (int i = 0; i < E::kPer; ++i) any |= v0 + i / E::kVec * kThreads < r.n_vec && top_bits(x[i]) > last;
+        for (int i = 0; i < E::kPer; ++i) {
+            const int v = v0 + i / E::kVec * kThreads;
+            any |= v < r.n_vec && top_key(x[i], r.lead + v * E::kVec + i % E::kVec) > last;
+        }
         if (!__syncthreads_or(any)) continue;
         int at = -1;  // the thread's first element of the largest bits
         uint32_t largest = 0;
