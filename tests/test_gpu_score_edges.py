@@ -61,3 +61,28 @@ def test_ties_with_the_ragged_end_of_a_row(vxk, dtype, n_top, rows, vocab):
     ids = _score_logits(vxk, l, dtype, vocab, torch.zeros(rows), n_top)[2]
     assert torch.equal(ids, _lowest_first(l, n_top))
     assert ids[0, 0] == 4096 and ids[1, 0] == 3 * 4096 + 5 and ids[2, 0] == 20000
+
+
+def _valid(ids, vocab):
+    ids = ids.cpu().numpy()
+    return ids.min() >= 0 and ids.max() < vocab and all(len(set(r)) == len(r) for r in ids)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [7, 600, 601, 4096, 4097, 30000])
+def test_lists_of_rows_with_hardly_a_number(vxk, dtype, vocab):
+    """NaN nearly everywhere: indices that exist and differ, the numbers first."""
+    import torch
+
+    nan, n_top = float("nan"), min(6, vocab)
+    l = torch.full((6, vocab), nan, device="cuda")
+    l[1, vocab - 1] = 1.0
+    l[2, vocab // 2] = -float("inf")
+    l[3, : vocab // 3] = 2.0
+    l[4, ::5] = -3.0
+    l[5, [2, 4]] = torch.tensor([1.0, 2.0], device="cuda")
+    l = l.to(_torch_type(dtype))
+    lp, ent, ids, _ = _score_logits(vxk, l, dtype, vocab, torch.zeros(6), n_top)
+    assert bool(torch.isnan(lp).all()) and bool(torch.isnan(ent).all())
+    assert _valid(ids, vocab)
+    assert ids[1, 0] == vocab - 1 and ids[2, 0] == vocab // 2 and ids[3, 0] == 0 and ids[5, :2].tolist() == [4, 2]

@@ -178,9 +178,10 @@ __global__ void __launch_bounds__(kThreads, 2) score_warp_kernel(const ScoreLogi
         float x[E::kPer];
         const float m = take_strip<DT, false>(r, r.body + (int64_t) v0 * 16, v0, 32, x);
         if (top.n_top) {
-            // every lane's largest element, or none where it has no element
+            // no less than any of a lane's elements; a maximum of -inf may also be that of NaNs,
+            // which stand below -inf in the list and so bound nothing
             const uint32_t largest = v0 < r.n_vec ? top_bits(m) : 0u;
-            if (top.low == 0ull) top.bound(largest);
+            if (top.low == 0ull) top.bound(m > -INFINITY ? largest : 0u);
             if (__any_sync(kAll, largest >= (uint32_t) (top.low >> 32))) {
 #pragma unroll
                 for (int j = 0; j < E::kLoads; ++j) {
