@@ -39,6 +39,18 @@ def _score_logits(vxk, l, dtype, vocab, tokens, n_top):
     return outs
 
 
+def _score(vxk, w, x, dtype, tokens, n_top):
+    import torch
+
+    head = vxk.Head(dim=x.shape[1], vocab=len(w), dtype=dtype)
+    outs = _outputs(len(x), n_top)
+    tok = torch.as_tensor(tokens, dtype=torch.int32, device="cuda")
+    head.score(w.data_ptr(), x.data_ptr(), len(x), tok.data_ptr(), n_top, *(o.data_ptr() for o in outs), _stream())
+    head.sync(_stream())
+    head.close()
+    return outs
+
+
 def _lowest_first(l, n_top):
     import torch
 
@@ -86,3 +98,24 @@ def test_lists_of_rows_with_hardly_a_number(vxk, dtype, vocab):
     assert bool(torch.isnan(lp).all()) and bool(torch.isnan(ent).all())
     assert _valid(ids, vocab)
     assert ids[1, 0] == vocab - 1 and ids[2, 0] == vocab // 2 and ids[3, 0] == 0 and ids[5, :2].tolist() == [4, 2]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n_top", [1, 2, 4, 16])
+@pytest.mark.parametrize("rows,vocab", [(1, 3001), (70, 40000), (200, 40000)])
+def test_lists_of_hidden_rows_over_a_matrix_with_nan(vxk, dtype, n_top, rows, vocab):
+    """Whole groups of W's rows NaN beside the largest logits: indices that exist and differ, the numbers first."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(vocab + rows)
+    t = _torch_type(dtype)
+    x = torch.rand(rows, 64, generator=g, device="cuda") + 0.5
+    w = torch.rand(vocab, 64, generator=g, device="cuda").to(t)
+    for numbers in ([], list(range(8)), list(range(16, 24)), list(range(0, vocab, 131)), [5, vocab - 1]):
+        broken = torch.full_like(w, float("nan"))
+        broken[numbers] = w[numbers]
+        lp, ent, ids, _ = _score(vxk, broken, x, dtype, torch.zeros(rows), n_top)
+        assert bool(torch.isnan(lp).all()) and bool(torch.isnan(ent).all())
+        assert _valid(ids, vocab)
+        first = min(n_top, len(numbers))
+        assert bool(torch.isin(ids[:, :first].cpu(), torch.tensor(numbers, dtype=torch.int32)).all())

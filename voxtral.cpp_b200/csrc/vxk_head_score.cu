@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                 // of all the row's logits: what is below it is in no list.
                 float sorted[16];
 #pragma unroll
-                for (int g = 0; g < 16; ++g) sorted[g] = most[g];
+                for (int g = 0; g < 16; ++g) sorted[g] = fmaxf(most[g], -INFINITY);  // NaN: no number
 #pragma unroll
                 for (int size = 2; size <= 16; size *= 2)
 #pragma unroll
