@@ -521,7 +521,12 @@ VXK_API vxk_status vxk_head_score_logits(vxk_head * head, const void * logits, v
  * products, the softmax statistics and the top lists are one kernel, and W is
  * read once per 2048 rows.  x is rounded to W's type as in
  * vxk_head_logits_argmax; the tensor cores' sums are moved to fp32 registers
- * every 512 columns (bf16) or 256 (f16), every 128 for up to 16 rows.
+ * every 512 columns (bf16) or 256 (f16), more often for short rows and for up
+ * to 16 of them.  The tensor cores drop what a step leaves below 2^-23 of its
+ * running sum: sums that 24 bits hold are exact, others about as far off as a
+ * plain fp32 sum.  The logits, and in a near tie the first of a list, may
+ * differ in the last places from vxk_head_logits_argmax's and with the number
+ * of rows in a call.
  *   w  [vocab][dim] f16 or bf16;  x [rows][dim] fp32;  device, 16-byte aligned
  * Everything else as in vxk_head_score_logits.
  */

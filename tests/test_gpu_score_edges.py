@@ -1,4 +1,9 @@
-"""Scores of logits and of hidden rows at the edges of their definition, through the C ABI."""
+"""Scores of logits and of hidden rows at the edges of their definition, through the C ABI.
+
+Tolerances.  U = 2^-24 is a rounding of fp32.  Where the logits are exact (sums of integers) their differences
+l - m are too, so a log probability is one rounding U |value| from exact behind the error of log s: at most L
+terms in one thread and a tree of joins, (L + 64) U.
+"""
 from __future__ import annotations
 
 import pytest
@@ -6,6 +11,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 F32, F16, BF16 = 0, 1, 30
+U = 2.0 ** -24
 
 
 def _stream():
@@ -119,3 +125,39 @@ def test_lists_of_hidden_rows_over_a_matrix_with_nan(vxk, dtype, n_top, rows, vo
         assert _valid(ids, vocab)
         first = min(n_top, len(numbers))
         assert bool(torch.isin(ids[:, :first].cpu(), torch.tensor(numbers, dtype=torch.int32)).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,dim", [(2, 4096), (17, 2048), (130, 4096), (40, 576)])
+@pytest.mark.parametrize("kind", ["few", "early", "dense"])
+def test_sums_that_are_exact_stay_exact(vxk, dtype, rows, dim, kind):
+    """Integer products whose sums need no more than 12 bits: no step of them rounds, so neither may the logits."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(rows + dim)
+    t, vocab, n_top = _torch_type(dtype), 2000, 8
+    w = torch.randint(-8, 9, (vocab, dim), generator=g, device="cuda").to(t)
+    x = torch.zeros(rows, dim, device="cuda")
+    if kind == "dense":
+        x = torch.randint(0, 2, (rows, dim), generator=g, device="cuda").float() * 2 - 1
+    else:
+        for r in range(rows):
+            at = torch.randperm(dim if kind == "few" else 64, generator=g, device="cuda")[:5]
+            x[r, at] = 16.0 * torch.randint(-3, 4, (5,), generator=g, device="cuda")
+            x[r, at[0]] = 48.0
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    lp, ent, ids, top = _score(vxk, w, x, dtype, tokens, n_top)
+    l = x.double() @ w.double().T
+    assert float(l.abs().max()) < 4096
+    want = torch.log_softmax(l, 1)
+    p = want.exp()
+    tol = (16 + 64) * U  # 2000 columns over the CTAs are a tile of 32 each, 16 of them a thread's
+
+    def near(got, to):
+        return bool(((got.double() - to).abs() <= tol + 1.01 * U * to.abs()).all())
+
+    assert torch.equal(ids, _lowest_first(l, n_top))
+    assert near(lp, want.gather(1, tokens[:, None])[:, 0])
+    assert near(top, want.gather(1, ids.long()))
+    t_s = (p * (l - l.amax(1, keepdim=True))).sum(1).abs()  # the entropy is log s + this
+    assert bool(((ent.double() + (p * want).sum(1)).abs() <= tol * (1 + 2 * t_s)).all())

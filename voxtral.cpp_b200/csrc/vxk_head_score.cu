@@ -18,10 +18,12 @@
 // every step: over 4096 columns the largest logits come out 6e-6 too small, and the
 // entropy 4e-5 off.  So a sum is taken out every 512 columns (bf16) or 256 (f16, whose
 // products have six bits more to lose), two accumulators in turn in TMEM, and added up
-// in fp32 registers: 128 columns a thread, eight epilogue warps.  What is dropped in
-// the mean (dropped_share) is given back, one FMA a logit: entropies of 700 rows of
-// 2048 columns are then 1.1e-6 off (bf16) or 2.5e-6 (f16) instead of 4.3e-6 and 4.9e-6;
-// a plain fp32 product's are 5e-6 off.
+// in fp32 registers: 128 columns a thread, eight epilogue warps (segment_of).  Entropies of
+// 700 rows of 2048 columns are then 4.3e-6 off (bf16) or 4.9e-6 (f16), a plain fp32
+// product's 5e-6.  What is dropped always makes a sum smaller in magnitude; giving its mean
+// back as a factor would halve these errors or better for rows like those measured, but
+// change sums of few columns or few bits, of which nothing was dropped, by up to 11
+// units in the last place.
 //
 // Measured (bf16): 100 rows x 131072 x 2048 102 us with lists of 4, 5.3 TB/s of W (93 without:
 // 5.8); 2000 rows x 131072 x 4096 1590 us, 1.35 PFLOP/s (without lists 1450, 1.48; a plain
@@ -74,23 +76,17 @@ struct Shape {
     static constexpr int kBars = kDrain + 1;
 };
 
-// Chunks summed in TMEM before they are moved to registers; 2 for up to kFewRows rows,
-// where that brings f16's error down to half and bf16's to two thirds and costs 0-3 %
-// (32 rows of f16: 6 %).  One chunk at a time is no more exact: the fp32 adds are then what
-// is left, a unit or two in a logit's last place.
+// Chunks summed in TMEM before they are moved to registers: 8 (bf16) or 4 (f16).  Where a plain
+// fp32 product is more exact than its usual few 1e-6 the segments are shorter.  Rows of fewer
+// than 1280 columns: at 1024, 2000 rows x 30000, 6 for 8 takes 153 us for 140 and brings an
+// entropy's error from 4.7e-6 to 3.2e-6 (bf16; plain 3.6e-6), 3 for 4 197 us for 170 and 5.4e-6 to
+// 3.5e-6 (f16; plain 4.2e-6).  Up to 16 rows, which a plain product sums in trees: 2, no slower
+// than 8, or 1 for up to four rows of f16 (2.2e-6 -> 1.2e-6, a unit or two in a logit's last
+// place; one row x 131072 x 2048 104 -> 130 us, x 32000 x 1280 28.7 -> 29.9).
 template <int DT>
-constexpr int kSegmentOf = DT == 30 ? 8 : 4;
-constexpr int kFewRows = 16;
-
-// What the accumulation drops of a sum on average, relative to it.  A step (16 columns)
-// truncates the running sum at 2^-23 of its power of two: half a unit of it is lost in the
-// mean, 2^-24 E[2^floor(log2 x) / x] = 2^-24 / (2 ln 2) of the running sum x, which over
-// the steps of a segment averages half of the segment's.
-__device__ __forceinline__ float dropped_share(int n_chunks, int segment) {
-    constexpr float kStep = 0.72134752f / (1 << 25);
-    const int whole = n_chunks / segment, rest = n_chunks % segment;
-    // segments weigh in by their columns
-    return kStep * 4.0f * (float) (whole * segment * segment + rest * rest) / (float) n_chunks;
+__device__ __forceinline__ int segment_of(int n_rows, int n_chunks) {
+    if (n_rows <= 16) return DT != 30 && n_rows <= 4 ? 1 : 2;
+    return DT == 30 ? min(8, max(1, n_chunks * 2 / 5)) : min(4, max(1, n_chunks / 5));
 }
 
 // One thread's list of its largest keys, largest first.  LIST 0: none; up to 4 places in
@@ -159,7 +155,6 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
                                                                  const __grid_constant__ CUtensorMap tmx,
                                                                  const HeadScoreParams p) {
     using S = Shape<CG>;
-    const int segment = p.n_rows <= kFewRows ? 2 : kSegmentOf<DT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t * base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned long long * lists = reinterpret_cast<unsigned long long *>(base + kRing);
@@ -173,6 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
     const int row_tile = unit % p.n_row_tiles, group = unit / p.n_row_tiles;
     const int row0 = row_tile * (128 * CG) + rank * 128;  // this CTA's first row
     const int n_chunks = p.dim / kChunk;
+    const int segment = segment_of<DT>(p.n_rows, n_chunks);
     const int n_segs = (n_chunks + segment - 1) / segment;
 
     if (tid == 0) {
@@ -289,7 +285,6 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
         const bool listed = LIST != 0 && row < p.n_rows;
         asm volatile("griddepcontrol.wait;" ::: "memory");
         const int32_t token = p.tokens && row < p.n_rows ? p.tokens[row] : -1;
-        const float dropped = dropped_share(n_chunks, segment);
         Stat a = stat_empty();
         uint32_t seg = 0;  // two accumulators in turn: bit 0, and the parity in bit 1
         bool have = true;
@@ -317,8 +312,6 @@ __global__ void __launch_bounds__(kThreads, 1) head_score_kernel(const __grid_co
             if (!rows_here) continue;
             // the row's bound so far, on its way while the statistics are taken
             uint32_t bound = listed && tile != group ? __ldcg(&p.row_low[row]) : 0u;
-#pragma unroll
-            for (int j = 0; j < kHalfCols; ++j) acc[j] = fmaf(acc[j], dropped, acc[j]);
             const int col0 = tile * p.tile_cols + half * n_half;
             const int limit = min(n_half, p.vocab - col0);
             if (limit < kHalfCols) {
