@@ -821,11 +821,14 @@ VXK_API vxk_status vxk_decoder_forward(vxk_decoder * d, const int32_t * tokens, 
  * token gives the log probability of given[r], its entropy and its n_top most
  * likely tokens (vxk_head_score; the outputs are its, per row).  With a
  * transcript's tokens and given[r] = tokens[r + 1] these are the transcript's
- * word confidences.  A batch of 64 rows or more whose streams all begin with
- * it is attended as packed prompts (vxk_prompt_attention, f16 rows), any other
- * one, or one of an F32 cache, over the cache (vxk_attend_layer); the caches
- * are appended as in vxk_decoder_forward and the caller commits, or aborts to
- * leave no trace.
+ * word confidences.  On an F16 cache a batch of 64 rows or more whose streams
+ * all begin with it is attended as packed prompts (vxk_prompt_attention, f16
+ * rows); any other batch, and every one on an F32 or Q8_0 cache, over the cache
+ * as in vxk_decoder_forward (vxk_attend_layer).  The packed form rounds q and the
+ * probabilities to f16, which the quantized products' rounding of their
+ * activations can carry to about 1 % of the largest logit: a prompt's scores may
+ * differ by that with what else is in its batch.  The caches are appended as in
+ * vxk_decoder_forward and the caller commits, or aborts to leave no trace.
  *   given  [rows] host array, < vocab; a negative one is not scored
  * Asynchronous on cuda_stream; the first call allocates its scratch.
  */

@@ -297,3 +297,38 @@ def test_the_operators_in_a_chain(vxk):
     assert bool(((lp.double() - ref).abs() <= tol).all())
     prompt.close()
     head.close()
+
+
+@pytest.mark.parametrize("cache", [8, 1], ids=["q8_0 cache", "f16 cache"])
+@pytest.mark.parametrize("lens", [[60, 11], [30, 25], [128]], ids=str)
+def test_scores_are_the_forwards_own(vxk, tmp_path, cache, lens):
+    """Whole prompts on both sides of the packed form's 64 rows against the logits that vxk_decoder_forward gives for
+    the same batch.  A Q8_0 cache is attended as it is stored, at every size; an f16 cache's packed rows differ from it
+    by roundings of q and the probabilities to f16, which one step of the products' activation rounding can carry to the
+    1e-2 level."""
+    import torch
+
+    _, pool, dec = _setup(vxk, tmp_path, 81, cache=cache)
+    rng = np.random.default_rng(12)
+    vocab, rows = dec.info["vocab"], sum(lens)
+    streams = [pool.open_stream() for _ in lens]
+    amax = torch.zeros(len(lens), dtype=torch.int32, device="cuda")
+    tokens = [int(t) for t in rng.integers(0, vocab, rows)]
+    given = [int(t) for t in rng.integers(0, vocab, rows)]
+    pool.plan(streams, lens, _stream())
+    lp, ent, ids, top = _score(dec, tokens, [0] * rows, given, 4)
+    pool.abort()
+    pool.plan(streams, lens, _stream())
+    logits = torch.empty(len(lens), vocab, device="cuda")
+    dec.forward(tokens, [0] * rows, amax.data_ptr(), logits.data_ptr(), cuda_stream=_stream())
+    dec.sync(_stream())
+    pool.commit()
+    l = logits.cpu().numpy().astype(np.float64)
+    want = _log_softmax(l)
+    bar = (EXACT_BAR if cache == 8 or rows < 64 else 2 * STEP_BAR) * np.abs(l).max()
+    for s, r in enumerate(np.cumsum(lens) - 1):
+        assert abs(lp[r] - want[s, given[r]]) <= bar
+        assert np.all(np.abs(top[r] - want[s, ids[r]]) <= bar)
+        assert abs(ent[r] + (np.exp(want[s]) * want[s]).sum()) <= bar
+    dec.close()
+    pool.close()

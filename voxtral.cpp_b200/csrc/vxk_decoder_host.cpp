@@ -589,16 +589,16 @@ constexpr int32_t kPackedRows = 64;
 
 // The scoring state of a decoder, allocated once.
 void need_score(vxk_decoder * d) {
-    if (d->prompt) return;
     const size_t R = (size_t) d->ps.max_rows;
     const size_t qdim = (size_t) d->ps.n_q * d->ps.head_dim, kvdim = (size_t) d->ps.n_kv * d->ps.head_dim;
-    if (!d->p16) d->p16 = dalloc<uint16_t>(d, R * 2 * (qdim + kvdim));
     if (!d->d_given) d->d_given = dalloc<int32_t>(d, R);
     if (d->head_q && !d->score_logits) {
         // the embeddings are read once per chunk
         d->score_chunk = std::min<int32_t>(d->chunk, 128);
         d->score_logits = dalloc<float>(d, (size_t) d->score_chunk * d->vocab);
     }
+    if (d->prompt || d->ps.dtype != VXK_DTYPE_F16) return;  // (see `packed`)
+    if (!d->p16) d->p16 = dalloc<uint16_t>(d, R * 2 * (qdim + kvdim));
     vxk_prompt_config c = vxk_prompt_default_config();
     c.device = d->ps.device;
     c.n_q_heads = d->ps.n_q;
@@ -652,11 +652,12 @@ void forward(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slot
             if (sc->given[r] >= d->vocab) dfail(VXK_STATUS_INVALID_ARGUMENT, "given token out of range");
         need_score(d);
         upload(d, sc->given, (size_t) rows * sizeof(int32_t), d->d_given, cs);
-        // Streams that begin with this batch attend its rows alone; an f32 cache asks for
-        // more than 16-bit rows.  A layer's attention over the cache (32 / 8 heads of 128)
+        // Streams that begin with this batch attend its rows alone, in f16 as an f16 cache
+        // would hold them; an f32 cache holds more of them and a q8_0 cache less, and a
+        // prompt's scores have to be those of the cache that it is decoded on.  A layer's attention over the cache (32 / 8 heads of 128)
         // against the packed one, of which 2-3 us are the widened rows: 2 rows 6 / 15 us,
         // 38 rows 16 / 17, 8 x 38 rows 41 / 17, 512 rows 105 / 25, 4000 rows 3050 / 155.
-        packed = rows >= kPackedRows && !bv.single_token && d->ps.dtype != VXK_DTYPE_F32;
+        packed = rows >= kPackedRows && !bv.single_token && d->ps.dtype == VXK_DTYPE_F16;
         std::vector<int32_t> lens;
         for (int32_t i = 0, r0 = 0; i < n_out; r0 = bv.last_rows[(size_t) i] + 1, ++i) {
             lens.push_back(bv.last_rows[(size_t) i] + 1 - r0);
