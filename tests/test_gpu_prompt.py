@@ -327,3 +327,26 @@ def test_rope(vxk, dtype, lens, first, heads, kv, dim):
     assert torch.equal(outs[2][:rows], v.to(t))
     assert all(bool((o[rows:] == 9.0).all()) for o in outs)
     prompt.close()
+
+
+def test_values_that_are_not_finite_among_many_items_of_one_tile(vxk):
+    """Items with two tiles, each followed by dozens of one tile in the same CTA: a V row that is not finite reaches the
+    rows that attend it and no others."""
+    import torch
+
+    lens, heads, kv, dtype = [64] * 160 + [20] * 2500, 8, 2, F16
+    q, k, v = make(lens, heads, kv, 64, dtype)
+    clean = attend(vxk, q, k, v, lens, dtype)
+    assert bool(torch.isfinite(clean.float()).all())
+    hit = torch.zeros(sum(lens), kv, dtype=torch.bool, device="cuda")
+    at = 0
+    for i, n in enumerate(lens):
+        if i % 7 == 0:
+            row = at + (13 * i) % n
+            v[row, i % kv, i % 64] = float("nan" if i % 2 else "inf")
+            hit[row: at + n, i % kv] = True
+        at += n
+    got = attend(vxk, q, k, v, lens, dtype)
+    hit = hit.repeat_interleave(heads // kv, 1)
+    assert torch.equal(got[~hit], clean[~hit])
+    assert bool((~torch.isfinite(got[hit].float())).any(-1).all())

@@ -54,7 +54,7 @@ constexpr int kThreads = 384;
 // Registers a thread after the split: 128 x 72 + 256 x 216 = 384 x 168, the launch's.
 constexpr int kRegsIssue = 72, kRegsSoftmax = 216;
 constexpr int kTile = 128;        // query rows and keys of a tile
-constexpr int kFlags = 16;        // items that the V warps may be ahead of the epilogue
+constexpr int kFlags = 16;        // a tile's items whose V flags are kept
 constexpr float kSlack = 8.0f;    // growth of c m that is let pass without a rescale
 
 template <int HD>
@@ -68,8 +68,15 @@ struct Shape {
                          kSFull = kQEmpty + 2, kPFull = kSFull + 2, kODone = kPFull + 4, kDrain = kODone + 2;
     static constexpr int kBars = kDrain + 1;
     static constexpr int kOffMisc = kOffBar + 8 * kBars;  // TMEM base, abort flag, V flags
-    static constexpr int kSmem = kOffMisc + 8 + 2 * kFlags * 4 + 1024;
+    static constexpr int kSmem = kOffMisc + 8 + 4 * kFlags * 4 + 1024;
 };
+// The V warps may write the flags of an item of tile s while its softmax warps have yet to read
+// those of an earlier one.  Counted in items that have a tile s, the writers are never more than
+// kStages / 2 + 1 ahead: the issuer passes such an item only with P, which those warps make
+// behind the epilogue of the one before, and the ring lets the V warps kStages tiles, two an item at
+// least, past the issuer.  (Counted in all items there would be no limit: those without a tile B do
+// not wait for its warps.)
+static_assert(Shape<128>::kStages / 2 + 1 < kFlags && Shape<64>::kStages / 2 + 1 < kFlags, "V flags overtake their readers");
 static_assert(Shape<128>::kSmem <= 232448 && Shape<64>::kSmem <= 232448, "attention exceeds 227 KB of shared memory");
 
 // What every role derives from an item.
@@ -331,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
     uint64_t * bars = reinterpret_cast<uint64_t *>(base + S::kOffBar);
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(base + S::kOffMisc);
     volatile int32_t * abort_flag = reinterpret_cast<volatile int32_t *>(base + S::kOffMisc + 4);
-    volatile int32_t * v_flags = reinterpret_cast<volatile int32_t *>(base + S::kOffMisc + 8);  // [2 warps][kFlags]
+    volatile int32_t * v_flags = reinterpret_cast<volatile int32_t *>(base + S::kOffMisc + 8);  // [2 tiles][2 warps][kFlags]
 
     const int tid = threadIdx.x, warp = (int) uniform(tid >> 5), lane = tid & 31;
     const int4 head = *reinterpret_cast<const int4 *>(p.plan);
@@ -520,6 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             // a wait by parity holds only for a reader that is never a turn of the ring away.
             const int t = (warp - 2) * 32 + lane;
             uint32_t st = 0, par = 0;
+            int nth[2] = {0, 0};  // items of either tile so far
             bool ok = true;
             for (int i = begin; ok && i < end; ++i) {
                 Item it;
@@ -548,11 +556,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         bad = __any_sync(0xffffffffu, bad);
-                        if (lane == 0) v_flags[(warp - 2) * kFlags + (i - begin) % kFlags] = bad;
+                        if (lane == 0) {
+#pragma unroll
+                            for (int s = 0; s < 2; ++s)
+                                if (it.n[s]) v_flags[(2 * s + warp - 2) * kFlags + nth[s] % kFlags] = bad;
+                        }
                     }
                     if (lane == 0) mbar_arrive(&bars[S::kReady + st]);
                     if (++st == S::kStages) st = 0, par ^= 1;
                 }
+                nth[0] += it.n[0] != 0;
+                nth[1] += it.n[1] != 0;
             }
         }
         __syncwarp();
@@ -565,6 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         const uint32_t ts = tmem + s * kTile + lanes, to = tmem + 2 * kTile + s * HD + lanes;
         const float c = p.scale_log2;
         uint32_t cs = 0;                                     // key tiles so far
+        int nth = 0;                                         // items of this tile so far
         bool ok = true;
         for (int i = begin; ok && i < end; ++i) {
             Item it;
@@ -605,7 +620,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             ok = __all_sync(0xffffffffu, tc_wait(&bars[S::kODone + s], (cs - 1) & 1, abort_flag, p.error));
             if (!ok) break;
             tc_fence_after();
-            const bool bad = v_flags[(i - begin) % kFlags] | v_flags[kFlags + (i - begin) % kFlags];
+            const bool bad = v_flags[2 * s * kFlags + nth % kFlags] | v_flags[(2 * s + 1) * kFlags + nth % kFlags];
+            ++nth;
             const int head = it.head + (r & ((1 << p.pack_shift) - 1));
             const float f = 1.0f / row.sum;
             uint16_t * out = static_cast<uint16_t *>(p.out) + ((int64_t) (it.row0 + token) * p.n_q + head) * HD;
