@@ -332,3 +332,33 @@ def test_scores_are_the_forwards_own(vxk, tmp_path, cache, lens):
         assert abs(ent[r] + (np.exp(want[s]) * want[s]).sum()) <= bar
     dec.close()
     pool.close()
+
+
+def test_a_decode_step_behind_a_scored_batch_waits_as_before(vxk, tmp_path):
+    """vxk_decoder_sync of a step that uses no packed attention makes the calls that it made before any was used."""
+    import torch
+    from torch.profiler import ProfilerActivity, profile
+
+    _, pool, dec = _setup(vxk, tmp_path, 91)
+    a = pool.open_stream()
+    amax = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def step():
+        pool.plan([a], [1], _stream())
+        dec.forward([7], [0], amax.data_ptr(), cuda_stream=_stream())
+        torch.cuda.synchronize()
+        with profile(activities=[ProfilerActivity.CUDA]) as p:
+            dec.sync(_stream())
+        pool.commit()
+        return sum(e.count for e in p.key_averages() if "Memcpy DtoH" in e.key)
+
+    step()
+    before = step()
+    assert before > 0
+    b = pool.open_stream()
+    pool.plan([b], [70], _stream())
+    _score(dec, [3] * 70, [0] * 70, [4] * 70, 0)
+    pool.commit()
+    assert step() == before
+    dec.close()
+    pool.close()

@@ -137,6 +137,8 @@ struct vxk_decoder {
     vxk::PoolBatchView view;
     // scoring, created by the first vxk_decoder_score
     vxk_prompt * prompt = nullptr;
+    bool prompt_used = false;      // since the last sync that looked at its error word
+    cudaStream_t prompt_stream = nullptr;  // the stream of that use
     uint16_t * p16 = nullptr;      // q, k, v and output rows of the packed attention
     int32_t * d_given = nullptr;   // [max_rows]
     float * score_logits = nullptr;  // [score_chunk][vocab], quantized heads only
@@ -663,7 +665,11 @@ void forward(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slot
             lens.push_back(bv.last_rows[(size_t) i] + 1 - r0);
             packed = packed && bv.row_pos[(size_t) r0] == 0;
         }
-        if (packed) VXK_DCALL(vxk_prompt_plan(d->prompt, lens.data(), nullptr, n_out, cs), "vxk_prompt_plan");
+        if (packed) {
+            d->prompt_used = true;
+            d->prompt_stream = cs;
+            VXK_DCALL(vxk_prompt_plan(d->prompt, lens.data(), nullptr, n_out, cs), "vxk_prompt_plan");
+        }
     }
     upload(d, d->h_rows.data(), (size_t) rows * sizeof(vxk::DecRow), d->d_rows, cs);
 
@@ -1012,9 +1018,11 @@ vxk_status vxk_decoder_sync(vxk_decoder * d, void * cuda_stream, int32_t timeout
     if (st != VXK_STATUS_OK) return st;
     st = vxk_head_sync(d->head, cuda_stream, timeout_ms);
     if (st != VXK_STATUS_OK) d->last_error = "head reported a device error";
-    if (st == VXK_STATUS_OK && d->prompt) {
+    if (st == VXK_STATUS_OK && d->prompt_used) {
         st = vxk_prompt_sync(d->prompt, cuda_stream, timeout_ms);
         if (st != VXK_STATUS_OK) d->last_error = "packed attention reported a device error";
+        // a wait for another stream says nothing of the packed batch
+        if (st != VXK_STATUS_TIMEOUT && d->prompt_stream == static_cast<cudaStream_t>(cuda_stream)) d->prompt_used = false;
     }
     return st;
 }
