@@ -161,3 +161,34 @@ def test_sums_that_are_exact_stay_exact(vxk, dtype, rows, dim, kind):
     assert near(top, want.gather(1, ids.long()))
     t_s = (p * (l - l.amax(1, keepdim=True))).sum(1).abs()  # the entropy is log s + this
     assert bool(((ent.double() + (p * want).sum(1)).abs() <= tol * (1 + 2 * t_s)).all())
+
+
+def test_the_first_call_of_a_head_waits_for_no_other_stream(vxk):
+    """Its scratch is allocated and cleared while another stream is busy for a second."""
+    import time
+
+    import torch
+
+    l = torch.randn(5, 9000, device="cuda")
+    tok = torch.zeros(5, dtype=torch.int32, device="cuda")
+    outs = _outputs(5, 3)
+    side = torch.cuda.Stream()
+
+    def call(head):
+        head.score_logits(l.data_ptr(), F32, 9000, 5, tok.data_ptr(), 3, *(o.data_ptr() for o in outs), side.cuda_stream)
+
+    warm, head = vxk.Head(dim=64, vocab=9000), vxk.Head(dim=64, vocab=9000)
+    call(warm)
+    torch.cuda.synchronize()
+    want = [o.clone() for o in outs]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(int(1.9e9))  # the legacy stream, about a second
+    t = time.perf_counter()
+    call(head)
+    took = time.perf_counter() - t
+    torch.cuda.synchronize()
+    busy = time.perf_counter() - t
+    assert busy > 0.4 and took < busy / 4, (took, busy)
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    warm.close()
+    head.close()

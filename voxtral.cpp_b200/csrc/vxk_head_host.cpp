@@ -159,7 +159,8 @@ void need_score_scratch(vxk_head * h, cudaStream_t cs) {
     const size_t xh = take((size_t) vxk::kScoreRows * h->cfg.dim * 2);
     uint8_t * base = nullptr;
     VXK_HCUDA(cudaMalloc(&base, at));
-    if (cudaMemset(base, 0, ctas * sizeof(int32_t)) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess) {
+    // on the call's own stream: a later call of this head has to be ordered behind this one anyway
+    if (cudaMemsetAsync(base, 0, ctas * sizeof(int32_t), cs) != cudaSuccess) {
         cudaFree(base);
         hfail(VXK_STATUS_BACKEND_ERROR, "clearing the scoring scratch failed");
     }
