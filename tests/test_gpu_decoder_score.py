@@ -362,3 +362,48 @@ def test_a_decode_step_behind_a_scored_batch_waits_as_before(vxk, tmp_path):
     assert step() == before
     dec.close()
     pool.close()
+
+
+def test_handles_of_their_own_on_several_threads(vxk):
+    """Eight host threads, each with a prompt, a head and a stream of its own, make and use them at once."""
+    import threading
+
+    import torch
+
+    lens, heads, dim, vocab = [40, 90], 4, 64, 5000
+    rows, width = sum(lens), heads * dim
+    torch.manual_seed(4)
+    q, k, v = (torch.randn(rows, n, dim, device="cuda").half() for n in (heads, 2, 2))
+    w, tokens = torch.randn(vocab, width, device="cuda").half(), torch.arange(rows, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    got, errors, start = [None] * 8, [], threading.Barrier(8)
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            out, x, lp = (torch.empty(n, dtype=t, device="cuda") for n, t in
+                          ((q.shape, torch.float16), ((rows, width), torch.float32), (rows, torch.float32)))
+            start.wait()
+            prompt = vxk.Prompt(n_q_heads=heads, n_kv_heads=2, head_dim=dim, max_seqs=2, max_rows=rows, max_position=0)
+            head = vxk.Head(dim=width, vocab=vocab)
+            prompt.plan(lens, cuda_stream=s.cuda_stream)
+            with torch.cuda.stream(s):
+                prompt.attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), s.cuda_stream)
+                x.copy_(out.reshape(rows, width))
+                head.score(w.data_ptr(), x.data_ptr(), rows, tokens.data_ptr(), 0, lp.data_ptr(), cuda_stream=s.cuda_stream)
+            prompt.sync(s.cuda_stream)
+            head.sync(s.cuda_stream)
+            got[i] = lp.cpu()
+            prompt.close()
+            head.close()
+        except Exception as e:  # noqa: BLE001 - reported by the test
+            errors.append(e)
+            start.abort()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    assert all(torch.equal(g, got[0]) for g in got) and bool(torch.isfinite(got[0]).all())

@@ -59,15 +59,15 @@ private:
 // so the library does not link libcuda.
 void encode_rows_map(CUtensorMap * map, const void * base, int32_t dtype, int64_t cols, int64_t rows,
                      int32_t box_rows) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    if (!encode) {
+    // looked up once, by whichever thread comes first
+    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
         void * fn = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
             q != cudaDriverEntryPointSuccess || !fn)
             hfail(VXK_STATUS_BACKEND_ERROR, "cuTensorMapEncodeTiled is not available");
-        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }();
     const cuuint64_t dims[2] = {(cuuint64_t) cols, (cuuint64_t) rows};
     const cuuint64_t strides[1] = {(cuuint64_t) cols * 2};
     const cuuint32_t box[2] = {64, (cuuint32_t) box_rows};

@@ -61,15 +61,15 @@ constexpr int32_t kKeyTile = 128;
 // box_heads x box_rows, 128-byte swizzle, zero fill behind the last row.
 void encode_heads_map(CUtensorMap * map, const void * base, const vxk_prompt_config & c, int32_t heads, int64_t rows,
                       int32_t box_heads, int32_t box_rows) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    if (!encode) {
+    // looked up once, by whichever thread comes first
+    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
         void * fn = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
             q != cudaDriverEntryPointSuccess || !fn)
             pfail(VXK_STATUS_BACKEND_ERROR, "cuTensorMapEncodeTiled is not available");
-        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }();
     const cuuint64_t dims[3] = {(cuuint64_t) c.head_dim, (cuuint64_t) heads, (cuuint64_t) rows};
     const cuuint64_t strides[2] = {(cuuint64_t) c.head_dim * 2, (cuuint64_t) c.head_dim * 2 * (cuuint64_t) heads};
     const cuuint32_t box[3] = {64, (cuuint32_t) box_heads, (cuuint32_t) box_rows};
