@@ -606,7 +606,10 @@ VXK_API vxk_status vxk_prompt_rope(vxk_prompt * prompt, const float * q, const f
  * sum_j softmax_j(scale q[i][h] . k[j][h']) v[j][h'] over the rows j that row i
  * attends (vxk_prompt_config), h' = h / (n_q_heads / n_kv_heads).  Scores,
  * softmax and sums are fp32; the probabilities are rounded to the prompt's type
- * for their product with v, and out is rounded once.
+ * for their product with v (bf16: by 2^-9 of themselves; f16: by 2^-12, or
+ * 2^-32 of the row's largest where that is more), and out is rounded once.  A
+ * value of v that is not finite makes its dim infinite or NaN in the rows that
+ * attend it and in no other.
  *   q, out [rows][n_q_heads][head_dim], k, v [rows][n_kv_heads][head_dim],
  *   16-bit, device, 16-byte aligned; out overlaps no input
  * Rows behind the plan's last are neither read for a result nor written.  No

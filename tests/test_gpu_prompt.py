@@ -350,3 +350,38 @@ def test_values_that_are_not_finite_among_many_items_of_one_tile(vxk):
     hit = hit.repeat_interleave(heads // kv, 1)
     assert torch.equal(got[~hit], clean[~hit])
     assert bool((~torch.isfinite(got[hit].float())).any(-1).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("depth", [9.0, 12.0, 15.0, 17.5])
+def test_many_small_probabilities_beside_a_large_one(vxk, dtype, dim, depth):
+    """One key far above thousands of others, whose probabilities e^-depth are below f16's normal range.
+
+    A probability is scaled before it is rounded so that the largest is at least 2^7; what f16 holds as a subnormal is
+    then 2^-25 - 7 of the largest off, n 2^-32 of the largest |v| in all, besides the errors of check_attention.
+    """
+    import torch
+
+    lens = [3000, 700]
+    q, k, v = make(lens, 4, 2, dim, dtype)
+    q.zero_()
+    q[..., 0] = dim ** 0.5
+    k.zero_()
+    k[:, :, 0] = -depth
+    v[:] = torch.rand(v.shape, device="cuda").to(v.dtype) + 0.5
+    at = 0
+    for n in lens:  # the first key of each: nearly all of the weight, and a v of 0
+        k[at], v[at] = 0.0, 0.0
+        at += n
+    out, at = attend(vxk, q, k, v, lens, dtype), 0
+    h = HALF[dtype]
+    for n in lens:
+        s = (q[at: at + n].double() * dim ** -0.5).transpose(0, 1) @ k[at: at + n].double().repeat_interleave(2, 1).permute(1, 2, 0)
+        p = torch.softmax(s.masked_fill(torch.ones(n, n, device="cuda").triu(1) > 0, -float("inf")), -1)
+        want = (p @ v[at: at + n].double().repeat_interleave(2, 1).transpose(0, 1)).transpose(0, 1)
+        d = 2 * U * (dim + 4) * depth
+        tol = 2.02 * h * want + (2 * d + 2 * U * n) * want + n * 2.0 ** -32 * 1.5 + 2.0 ** -25
+        off = (out[at: at + n].double() - want).abs()
+        assert bool((off <= tol).all()), float((off / tol).max())
+        at += n

@@ -17,8 +17,8 @@
 // one tile's softmax runs, the tensor cores work for the other.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 (p is then at most
-// 2^8, inside f16 and as exact there as below 1): a few times a row instead of once a
-// tile.  Sums are fp32 over the unrounded p; p is rounded to the 16-bit type for its
+// 2^8, or 2^15 in f16, whose small p are lifted out of its subnormals): a few times a row
+// instead of once a tile.  Sums are fp32 over the unrounded p; p is rounded to the 16-bit type for its
 // product, which is the error that the format allows (2^-12 f16, 2^-9 bf16 on average).
 //
 // Bound by the exponentials and the tensor cores together: a 128 x 128 tile of head dim 128
@@ -56,6 +56,11 @@ constexpr int kRegsIssue = 72, kRegsSoftmax = 216;
 constexpr int kTile = 128;        // query rows and keys of a tile
 constexpr int kFlags = 16;        // a tile's items whose V flags are kept
 constexpr float kSlack = 8.0f;    // growth of c m that is let pass without a rescale
+// p is made 2^kLift times as large, in the sums too: f16 then holds it to 2^-11 of itself down to
+// 2^-21 of the largest and to 2^-32 of that below, and 2^(kSlack + kLift) is still inside its
+// range.  Unlifted, thousands of keys at 2^-25 of the largest would come to nothing.
+template <int DT>
+constexpr float kLift = DT == 30 ? 0.0f : 7.0f;
 
 template <int HD>
 struct Shape {
@@ -237,7 +242,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// p = 2^(c x + off) of 32 scores, added to the sums and stored as 16 bits in TMEM.
+// p = 2^(c x + off) of 32 scores (off: kLift - c m), added to the sums and stored as 16 bits in TMEM.
 template <int DT>
 __device__ __forceinline__ void exp_chunk(const float * x, uint32_t tp, uint64_t c2, uint64_t off2, uint64_t (&total)[2]) {
     uint32_t h[16];
@@ -308,7 +313,7 @@ __device__ __forceinline__ void tile_step(float (&x)[128], uint32_t tp, float c,
         grown(f);
     }
     if (r.m == -INFINITY) r.m = mn;                  // nothing in O or the sum yet
-    const float off = r.m == -INFINITY ? 0.0f : -r.m * c;
+    const float off = r.m == -INFINITY ? 0.0f : fmaf(-r.m, c, kLift<DT>);
     const uint64_t c2 = pair(c, c), off2 = pair(off, off);
     uint64_t total[2] = {0, 0};
 #pragma unroll
