@@ -833,7 +833,8 @@ VXK_API vxk_status vxk_decoder_forward(vxk_decoder * d, const int32_t * tokens, 
  * differ by that with what else is in its batch.  The caches are appended as in
  * vxk_decoder_forward and the caller commits, or aborts to leave no trace.
  *   given  [rows] host array, < vocab; a negative one is not scored
- * Asynchronous on cuda_stream; the first call allocates its scratch.
+ * Asynchronous on cuda_stream; the first call allocates its scratch.  Refused
+ * inside a stream capture: a replay would not read the host arrays again.
  */
 VXK_API vxk_status vxk_decoder_score(vxk_decoder * d, const int32_t * tokens, const int32_t * audio_slots,
                                      const int32_t * given, int32_t n_top, float * logprob, float * entropy,

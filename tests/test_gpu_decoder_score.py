@@ -407,3 +407,26 @@ def test_handles_of_their_own_on_several_threads(vxk):
         t.join()
     assert not errors
     assert all(torch.equal(g, got[0]) for g in got) and bool(torch.isfinite(got[0]).all())
+
+
+def test_scoring_inside_a_capture_is_refused(vxk, tmp_path):
+    """It uploads what the host gives it, which a replay would not do again: refused, and usable afterwards."""
+    import torch
+
+    _, pool, dec = _setup(vxk, tmp_path, 95)
+    a = pool.open_stream()
+    side = torch.cuda.Stream()
+    for rows in (2, 70):
+        for warm in (False, True):
+            pool.plan([a], [rows], _stream())
+            torch.cuda.synchronize()
+            with pytest.raises(vxk.VxkError) as e:
+                with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                    dec.score([3] * rows, [0] * rows, [4] * rows, 0, cuda_stream=torch.cuda.current_stream().cuda_stream)
+            assert e.value.status == vxk.INVALID_STATE
+            first = _score(dec, [3] * rows, [0] * rows, [4] * rows, 2)
+            again = _score(dec, [3] * rows, [0] * rows, [4] * rows, 2)
+            assert all(np.array_equal(x, y) for x, y in zip(first, again))
+            pool.abort()
+    dec.close()
+    pool.close()

@@ -918,6 +918,10 @@ vxk_status vxk_decoder_score(vxk_decoder * d, const int32_t * tokens, const int3
         if (!given) dfail(VXK_STATUS_INVALID_ARGUMENT, "null argument");
         if (n_top < 0 || n_top > vxk::kMaxTop || n_top > d->vocab)
             dfail(VXK_STATUS_INVALID_ARGUMENT, "n_top must be in [0, min(16, vocab)]");
+        DevScope scope(d->ps.device);
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        VXK_DCUDA(cudaStreamIsCapturing(static_cast<cudaStream_t>(cuda_stream), &capture));
+        if (capture != cudaStreamCaptureStatusNone) dfail(VXK_STATUS_INVALID_STATE, "vxk_decoder_score inside a stream capture");
         const ScoreCall sc{given, n_top, logprob, entropy, top_ids, top_logprobs};
         forward(d, tokens, audio_slots, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(cuda_stream), &sc);
     });
