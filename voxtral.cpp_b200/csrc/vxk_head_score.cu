@@ -25,9 +25,11 @@
 // change sums of few columns or few bits, of which nothing was dropped, by up to 11
 // units in the last place.
 //
-// Measured (bf16): 100 rows x 131072 x 2048 102 us with lists of 4, 5.3 TB/s of W (93 without:
-// 5.8); 2000 rows x 131072 x 4096 1590 us, 1.35 PFLOP/s (without lists 1450, 1.48; a plain
-// library product reaches 1.66 in a burst and 1.39 under the power cap); 5 rows of f16 x
+// Measured (bf16) in short runs (in brackets: back to back, under the power cap): 100 rows x
+// 131072 x 2048 102 us with lists of 4, 5.3 TB/s of W (112; 93 without lists); 2000 rows x
+// 131072 x 4096 1590 us, 1.35 PFLOP/s (1700; without lists 1450, 1.48; a plain library product
+// reaches 1.66 in a burst and 1.39 under the power cap), of f16, whose segments are half as
+// long, 2000 (2110: the TMEM reads); 5 rows of f16 x
 // 32000 x 1280 29 us, of which three launches and the join are 14.  The lists' cost
 // is the few candidates behind each row's bound, looked for by every thread of a tile.
 //

@@ -21,13 +21,14 @@
 // instead of once a tile.  Sums are fp32 over the unrounded p; p is rounded to the 16-bit type for its
 // product, which is the error that the format allows (2^-12 f16, 2^-9 bf16 on average).
 //
-// Bound by the exponentials and the tensor cores together: a 128 x 128 tile of head dim 128
-// is 512 clocks of matrix instructions and 1024 of ex2 (16 a clock and SM), which have to run
-// for one tile while the other's maxima, masks and conversions take the issue slots.  Measured,
-// 32 / 8 heads of 128: 8192 rows causal f16 484 us, 1.14 PFLOP/s (the exponentials alone are
-// 245 us, the products 330); sixteen ragged prompts of 9,935 rows, bf16, 138 us, 0.82; 64 x
-// 38 rows 24 us, where filling and emptying the pipeline is all; four times 1500 rows of 20
-// heads of 64, not causal, 93 us (exponentials 41).  A CTA's first scores of an item wait for
+// Bound by the waits from one step of a tile to the next: a 128 x 128 tile of head dim 128 is
+// 1024 clocks of matrix instructions (512 for either product) and 1024 of ex2 (16 a clock and
+// SM), and at 8192 rows both pipes are busy a little over half the time, the issue slots a third.
+// Measured in short runs (in brackets: back to back, under the power cap), 32 / 8 heads of
+// 128: 8192 rows causal f16 484 us, 1.14 PFLOP/s (550; the exponentials alone are 245 us, the
+// products 330); sixteen ragged prompts of 9,935 rows, bf16, 138 us, 0.82 (153); 64 x 38 rows
+// 24.6 us, where filling and emptying the pipeline is all; four times 1500 rows of 20 heads
+// of 64, not causal, 94 us (exponentials 41).  A CTA's first scores of an item wait for
 // its Q, and an item's end (the last product, the division, 64 KB of output) is 3500 clocks,
 // about 2.5 us of 15 an item in the ragged case.
 //
